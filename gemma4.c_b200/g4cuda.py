@@ -28,6 +28,7 @@ ERRORS = {-1: "G4_ERR_INVALID", -2: "G4_ERR_FORMAT", -3: "G4_ERR_CUDA", -4: "G4_
           -5: "G4_ERR_DEVICE", -6: "G4_ERR_STATE"}
 OPT_GRAPHS, OPT_PDL, OPT_GEMM_PATH, OPT_LAYERS, OPT_STRICT, OPT_PERSISTENT, OPT_BATCH_SPLITS = 1, 2, 3, 4, 5, 6, 7
 SYN_GROUP_SCALES, SYN_RANDOM_NORMS = 1, 2
+TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2
 
 _f32p = np.ctypeslib.ndpointer(np.float32, flags="C_CONTIGUOUS")
 _i8p = np.ctypeslib.ndpointer(np.int8, flags="C_CONTIGUOUS")
@@ -39,6 +40,18 @@ class G4Error(RuntimeError):
     def __init__(self, code, msg=""):
         self.code = code
         super().__init__(f"{ERRORS.get(code, code)}: {msg}")
+
+
+class Kv4Cache(C.Structure):
+    """g4_kv4_cache: a pool of 4-bit KV pages (`pages`: its device address)."""
+    _fields_ = [("pages", C.c_void_p), ("num_pages", C.c_int), ("page_size", C.c_int), ("kv_heads", C.c_int),
+                ("head_dim", C.c_int)]
+
+
+class Kv4Batch(C.Structure):
+    """g4_kv4_batch: whose the token rows are; the arrays are device addresses of int32."""
+    _fields_ = [("n", C.c_int), ("rows", C.c_int), ("offsets", C.c_void_p), ("start_pos", C.c_void_p),
+                ("page_table", C.c_void_p), ("table_stride", C.c_int)]
 
 
 _lib = None
@@ -103,6 +116,18 @@ def load(path=LIB_PATH):
     L.g4_seq_alloc.argtypes = [vp, C.c_int, C.c_int]
     L.g4_forward_batch.argtypes = [vp, C.c_int, _i32p, _i32p, _i32p, _i32p]
     L.g4_logits_batch.argtypes = [vp, vp, vp]
+    i64, u64, cache, batch = C.c_int64, C.c_uint64, C.POINTER(Kv4Cache), C.POINTER(Kv4Batch)
+    L.g4_kv4_page_bytes.argtypes = [C.c_int] * 3
+    L.g4_kv4_page_bytes.restype = u64
+    L.g4_kv4_write.argtypes = [cache, batch, C.c_int, vp, i64, vp, i64, vp]
+    L.g4_kv4_read.argtypes = [cache, batch, C.c_int, vp, i64, vp, i64, vp]
+    L.g4_kv4_attention_workspace.argtypes = [cache, batch, C.c_int, C.c_int]
+    L.g4_kv4_attention_workspace.restype = u64
+    L.g4_kv4_attention.argtypes = [cache, batch, C.c_int, C.c_int, vp, i64, vp, i64, C.c_float, C.c_int, vp, u64, vp]
+    L.g4_beam_workspace.argtypes = [C.c_int] * 3
+    L.g4_beam_workspace.restype = u64
+    L.g4_beam_select.argtypes = [C.c_int] * 4 + [vp, i64, vp, vp, C.c_int, vp, vp, vp, vp, vp, u64, vp]
+    L.g4_kv4_reorder.argtypes = [cache] + [C.c_int] * 3 + [vp] * 4 + [C.c_int, vp, vp, vp]
     _lib = L
     return L
 
@@ -291,6 +316,68 @@ class Model:
 
     def __exit__(self, *exc):
         self.close()
+
+
+# ---------------------------------------------------------------------------
+# 4-bit KV cache and beam search: device addresses in and out (include/g4cuda.h
+# has the semantics), enqueued on `stream` (a cudaStream_t as an integer; None:
+# the default stream), nothing allocated, no synchronisation
+
+def kv4_page_bytes(kv_heads, head_dim, page_size):
+    """Bytes of one page; 0 for a geometry that is not supported."""
+    return load().g4_kv4_page_bytes(kv_heads, head_dim, page_size)
+
+
+def kv4_write(cache, batch, dtype, k, k_stride, v, v_stride, stream=None):
+    """Quantise the rows' keys and values ([rows][kv_heads][head_dim]) into their pages."""
+    _check(load().g4_kv4_write(cache, batch, dtype, k, k_stride, v, v_stride, stream))
+
+
+def kv4_read(cache, batch, dtype, k, k_stride, v, v_stride, stream=None):
+    """Read the rows' keys and values back."""
+    _check(load().g4_kv4_read(cache, batch, dtype, k, k_stride, v, v_stride, stream))
+
+
+def kv4_attention_workspace(cache, batch, dtype, q_heads):
+    """Workspace bytes of kv4_attention; raises for shapes that it refuses."""
+    n = load().g4_kv4_attention_workspace(cache, batch, dtype, q_heads)
+    if n == 0:
+        raise G4Error(-1, "kv4_attention: bad cache, batch, type or head count")
+    return n
+
+
+def kv4_attention(cache, batch, dtype, q_heads, q, q_stride, out, out_stride, scale, window, workspace,
+                  workspace_bytes, stream=None):
+    """Attention of the rows' queries over their sequences' cached keys and values."""
+    _check(load().g4_kv4_attention(cache, batch, dtype, q_heads, q, q_stride, out, out_stride, scale, window,
+                                   workspace, workspace_bytes, stream))
+
+
+def beam_workspace(groups, beams, vocab):
+    """Workspace bytes of beam_select; raises for sizes that it refuses."""
+    n = load().g4_beam_workspace(groups, beams, vocab)
+    if n == 0:
+        raise G4Error(-1, "beam_select: bad groups, beams or vocab")
+    return n
+
+
+def beam_select(groups, beams, vocab, dtype, logits, logits_stride, scores, finished, eos, out_scores, parents,
+                tokens, out_finished, workspace, workspace_bytes, stream=None):
+    """One step of beam search: the best candidates over beams and vocabulary."""
+    _check(load().g4_beam_select(groups, beams, vocab, dtype, logits, logits_stride, scores, finished, eos,
+                                 out_scores, parents, tokens, out_finished, workspace, workspace_bytes, stream))
+
+
+def kv4_caches(caches):
+    """The caches of several layers as kv4_reorder takes them."""
+    return (Kv4Cache * len(caches))(*caches)
+
+
+def kv4_reorder(caches, groups, beams, parents, lengths, table_in, table_out, table_stride, spare_in, spare_out,
+                stream=None):
+    """Let the caches of groups x beams sequences follow the selected parents."""
+    _check(load().g4_kv4_reorder(caches, len(caches), groups, beams, parents, lengths, table_in, table_out,
+                                 table_stride, spare_in, spare_out, stream))
 
 
 # ---------------------------------------------------------------------------

@@ -110,6 +110,122 @@ int g4_set_seed(g4_ctx *ctx, uint64_t seed);
  * of its own two kernels is returned as G4_ERR_CUDA. */
 int g4_topk_noalloc(const float *logits, int n, int k, float *values, int *ids, void *stream);
 
+/* ---- 4-bit KV cache and beam search (hosts that own their device memory) ----
+ * No counterpart in the reference (fp32 rings, one sequence, no beams). Like
+ * g4_topk_noalloc these calls need no context: they take device pointers,
+ * allocate nothing, enqueue on `stream` (a cudaStream_t; NULL = the default
+ * stream) and return without synchronising, so they can be captured into a
+ * CUDA graph. They run on the device that holds `pages` (g4_beam_select: the
+ * logits) whichever device is current; `stream` and every other pointer must
+ * belong to it. A bad argument returns G4_ERR_INVALID before any GPU work; a
+ * pointer that is not device memory is one. What the kernels read from device
+ * memory (offsets, positions, page numbers, parents) is checked there: a page
+ * number outside [0, num_pages) is "no page", its tokens are neither written
+ * nor seen.
+ *
+ * The cache is a pool of pages. A page holds page_size consecutive tokens of
+ * one sequence for every kv head, in 4 bits: per token, head and group of 64
+ * dimensions codes c in -7..7 and a bf16 scale, standing for c * scale.
+ * Quantisation (no counterpart; the symmetric form of quantize,
+ * gemma4.c:265-279): scale = bf16(max|x| / 7), c = x / scale rounded to the
+ * nearest integer, ties to even; both exactly, as if computed in infinite
+ * precision. A group whose max|x| is below 2^-100 stores zeros; one with a
+ * value that is not finite, or 2^127 or more, reads back as NaN.
+ * Bytes of a page: for each kv head page_size / 16 records of 16 tokens, each
+ * 17 * head_dim bytes; with G = head_dim / 64, t the token in the record and d
+ * the dimension in its group (the low nibble of a byte first, n = c + 8):
+ *   K codes  [G][t & 7][d / 16][t >> 3][8 bytes: d & 15]     8 * head_dim bytes
+ *   V codes  [G][d / 8][t >> 1 & 3][t >> 3][t & 1][4 bytes: d & 7]   the same
+ *   K scales [t][G] bf16;  V scales [G][t >> 1 & 3][t >> 3][t & 1] bf16
+ * The order is the one in which a warp's tensor-core operands read it.
+ * A page pool needs no initialisation: only written tokens are read. */
+#define G4_TYPE_F32 0
+#define G4_TYPE_BF16 1
+#define G4_TYPE_F16 2
+
+typedef struct g4_kv4_cache {
+    void *pages;       /* num_pages * g4_kv4_page_bytes(...) bytes, 16-byte aligned */
+    int num_pages;
+    int page_size;     /* tokens per page: a power of two, 16..1024 */
+    int kv_heads;      /* 1..256 */
+    int head_dim;      /* 64, 128, 256 or 512 */
+} g4_kv4_cache;
+
+/* Token rows of n sequences (n and rows may be 0): rows offsets[i] ..
+ * offsets[i + 1] - 1 of the tensors belong to sequence i, at positions
+ * start_pos[i], start_pos[i] + 1, ... Position p of sequence i lies in page
+ * page_table[i * table_stride + p / page_size]. Rows at negative positions are
+ * padding (left-padded batches), rows from offsets[n] on belong to nobody. */
+typedef struct g4_kv4_batch {
+    int n;                    /* sequences, 0..65536 */
+    int rows;                 /* token rows of the tensors, 0..4194304; offsets are clamped to it */
+    const int *offsets;       /* device, [n + 1], ascending */
+    const int *start_pos;     /* device, [n] */
+    const int *page_table;    /* device, [n][table_stride] */
+    int table_stride;
+} g4_kv4_batch;
+
+/* Bytes of one page, 0 for a geometry that is not supported. */
+uint64_t g4_kv4_page_bytes(int kv_heads, int head_dim, int page_size);
+/* Quantise the rows' keys and values into their pages. k and v: `type` values
+ * [rows][kv_heads][head_dim], a row k_stride / v_stride elements after the one
+ * before it (16-byte aligned rows). Rows without a page are dropped. No two
+ * rows of a call may name the same slot of a page. */
+int g4_kv4_write(const g4_kv4_cache *cache, const g4_kv4_batch *batch, int type, const void *k, int64_t k_stride,
+                 const void *v, int64_t v_stride, void *stream);
+/* Read the rows' keys and values back (c * scale, rounded to `type`). Rows
+ * without a page read as 0; rows from offsets[n] on are left as they were. */
+int g4_kv4_read(const g4_kv4_cache *cache, const g4_kv4_batch *batch, int type, void *k, int64_t k_stride, void *v,
+                int64_t v_stride, void *stream);
+/* Attention of the rows' queries over their sequences' cached keys and values,
+ * the rows' own included (write them first): q, out [rows][q_heads][head_dim]
+ * of `type`, q_heads a multiple of kv_heads (head h reads kv head
+ * h * kv_heads / q_heads), at most 64 times it. The query at position p sees the keys 0..p,
+ * with window > 0 only those above p - window: out = softmax(scale * q.k) v.
+ * A row that sees no key (padding, no pages) gets 0; rows from offsets[n] on
+ * are left as they were. Scores, softmax statistics and sums are fp32; q keeps
+ * 22 significant bits, the probabilities 16.
+ * `workspace` (g4_kv4_attention_workspace bytes, 16-byte aligned, any content)
+ * is scratch of this call alone: calls that may overlap on the GPU (other
+ * streams, other captured graphs) need their own. */
+uint64_t g4_kv4_attention_workspace(const g4_kv4_cache *cache, const g4_kv4_batch *batch, int type, int q_heads);
+int g4_kv4_attention(const g4_kv4_cache *cache, const g4_kv4_batch *batch, int type, int q_heads, const void *q,
+                     int64_t q_stride, void *out, int64_t out_stride, float scale, int window, void *workspace,
+                     uint64_t workspace_bytes, void *stream);
+
+/* One step of `groups` beam searches of `beams` beams (1..32): of the beams x
+ * vocab candidates of a group, scored scores[beam] + log softmax(logits of the
+ * beam)[token], the `beams` best, best first, ties to the lower beam, then the
+ * lower token. logits: `type` [groups * beams][vocab], rows logits_stride
+ * elements apart. A beam whose `finished` flag is set (NULL: none) has one
+ * candidate, the token eos at its score; eos < 0: none ends a beam (then
+ * finished must be NULL). A candidate that is not a number, or of a beam whose
+ * score is not finite, counts as -inf; a logit that is NaN as -inf.
+ * out_scores / parents / tokens / out_finished (may be NULL): [groups][beams],
+ * not overlapping the inputs; parents count within the group, out_finished is
+ * the parent's flag or token == eos. The softmax's sum and the scores are
+ * joined in fp64. workspace: g4_beam_workspace bytes, 16-byte aligned, any
+ * content, scratch of this call alone. */
+uint64_t g4_beam_workspace(int groups, int beams, int vocab);
+int g4_beam_select(int groups, int beams, int vocab, int type, const void *logits, int64_t logits_stride,
+                   const float *scores, const unsigned char *finished, int eos, float *out_scores, int *parents,
+                   int *tokens, unsigned char *out_finished, void *workspace, uint64_t workspace_bytes, void *stream);
+/* Let the caches of groups x beams sequences follow `parents` (g4_beam_select;
+ * a parent outside [0, beams) counts as the beam itself). All beams of group g
+ * hold lengths[g] tokens. Pages that are full are shared: beam i takes its
+ * parent's entries for them. Of a page that is part full (lengths[g] %
+ * page_size tokens) every beam has its own: a beam with another parent gets
+ * its spare page, into which the records of 16 tokens that hold the parent's
+ * tokens are copied in each of the `layers` caches (1..64, same page size and
+ * count; one table for all), and its former page becomes its spare one.
+ * Entries after those stay the beam's own, so a beam needs its own page for
+ * every page_size tokens it generates, and one to spare. Tables:
+ * [groups * beams][table_stride], spare pages [groups * beams]; the outputs
+ * must not overlap the inputs. */
+int g4_kv4_reorder(const g4_kv4_cache *caches, int layers, int groups, int beams, const int *parents,
+                   const int *lengths, const int *table_in, int *table_out, int table_stride, const int *spare_in,
+                   int *spare_out, void *stream);
+
 /* Wait for queued work; returns any device-side error. */
 int g4_sync(g4_ctx *ctx);
 

@@ -1,0 +1,145 @@
+"""The 4-bit cache and beam search on the CPU: sizes and refusals (every bad
+argument is refused before any GPU work), and the reference's own layout."""
+
+import numpy as np
+import pytest
+
+import kv4_ref as ref
+
+P = 0x10000          # an aligned address that no refused call may touch
+
+
+def cache(g4, **kw):
+    d = dict(pages=P, num_pages=4, page_size=64, kv_heads=1, head_dim=256)
+    d.update(kw)
+    return g4.Kv4Cache(**d)
+
+
+def batch(g4, **kw):
+    d = dict(n=2, rows=8, offsets=P, start_pos=P, page_table=P, table_stride=4)
+    d.update(kw)
+    return g4.Kv4Batch(**d)
+
+
+BAD_CACHE = [dict(pages=None), dict(pages=P + 8), dict(num_pages=0), dict(page_size=24), dict(page_size=8),
+             dict(page_size=2048), dict(page_size=0), dict(kv_heads=0), dict(kv_heads=257), dict(head_dim=96),
+             dict(head_dim=0), dict(head_dim=1024)]
+BAD_BATCH = [dict(n=-1), dict(n=65537), dict(rows=-1), dict(rows=(1 << 22) + 1), dict(offsets=None),
+             dict(start_pos=None), dict(page_table=None), dict(offsets=P + 2), dict(page_table=P + 1),
+             dict(table_stride=0)]
+
+
+def test_page_bytes(g4):
+    assert g4.kv4_page_bytes(1, 256, 64) == 64 // 16 * 17 * 256
+    assert g4.kv4_page_bytes(8, 128, 16) == 8 * 17 * 128
+    for bad in ((0, 64, 64), (1, 65, 64), (1, 64, 48), (1, 64, 8), (300, 64, 64)):
+        assert g4.kv4_page_bytes(*bad) == 0
+
+
+@pytest.mark.parametrize("name", ["g4_kv4_write", "g4_kv4_read"])
+def test_move_refusals(g4, name):
+    f = getattr(g4.load(), name)
+
+    def call(c=None, b=None, kind=0, k=P, ks=256, v=P, vs=256):
+        return f(c or cache(g4), b or batch(g4), kind, k, ks, v, vs, None)
+    for kw in BAD_CACHE:
+        assert call(c=cache(g4, **kw)) == -1, kw
+    for kw in BAD_BATCH:
+        assert call(b=batch(g4, **kw)) == -1, kw
+    for kw in (dict(kind=3), dict(kind=-1), dict(k=None), dict(v=None), dict(k=P + 4), dict(ks=255), dict(vs=258),
+               dict(ks=-256), dict(kind=1, ks=260), dict(ks=1 << 50)):
+        assert call(**kw) == -1, kw
+    assert f(None, batch(g4), 0, P, 256, P, 256, None) == -1
+    assert f(cache(g4), None, 0, P, 256, P, 256, None) == -1
+    # nothing to do: no GPU work
+    assert call(b=batch(g4, n=0)) == 0 and call(b=batch(g4, rows=0)) == 0
+
+
+def test_attention_refusals(g4):
+    f = g4.load().g4_kv4_attention
+
+    def call(c=None, b=None, kind=0, heads=8, q=P, qs=2048, o=P, os=2048, scale=1.0, window=0, ws=P, wb=1 << 40):
+        return f(c or cache(g4), b or batch(g4), kind, heads, q, qs, o, os, scale, window, ws, wb, None)
+    for kw in BAD_CACHE:
+        assert call(c=cache(g4, **kw)) == -1, kw
+    for kw in BAD_BATCH:
+        assert call(b=batch(g4, **kw)) == -1, kw
+    for kw in (dict(kind=9), dict(heads=0), dict(heads=-8), dict(c=cache(g4, kv_heads=3)), dict(heads=65, qs=65 * 256),
+               dict(q=None), dict(o=None), dict(q=P + 2), dict(qs=2047), dict(os=2050), dict(scale=float("nan")),
+               dict(scale=float("inf")), dict(window=-1), dict(ws=None), dict(ws=P + 8), dict(wb=0)):
+        assert call(**kw) == -1, kw
+    assert call(b=batch(g4, n=0)) == 0 and call(b=batch(g4, rows=0)) == 0
+    with pytest.raises(g4.G4Error):
+        g4.kv4_attention_workspace(cache(g4), batch(g4), 0, 7 * 64 + 1 + 64)
+    assert g4.kv4_attention_workspace(cache(g4), batch(g4), 0, 8) > 0
+
+
+def test_beam_refusals(g4):
+    f = g4.load().g4_beam_select
+
+    def call(g=1, w=4, v=1000, kind=0, x=P, xs=1000, s=P, fin=None, eos=-1, os=P, pa=P, to=P, fo=None, ws=P,
+             wb=1 << 40):
+        return f(g, w, v, kind, x, xs, s, fin, eos, os, pa, to, fo, ws, wb, None)
+    for kw in (dict(g=-1), dict(g=65537), dict(w=0), dict(w=33), dict(v=0), dict(v=(1 << 24) + 1), dict(kind=3),
+               dict(x=None), dict(x=P + 2), dict(kind=1, x=P + 1), dict(xs=999), dict(s=None), dict(s=P + 2),
+               dict(eos=1000), dict(fin=P), dict(os=None), dict(pa=None), dict(to=None), dict(ws=None),
+               dict(ws=P + 4), dict(wb=8)):
+        assert call(**kw) == -1, kw
+    assert call(g=0) == 0
+    for bad in ((1, 0, 10), (1, 33, 10), (1, 4, 0), (-1, 4, 10)):
+        assert g4.load().g4_beam_workspace(*bad) == 0
+        with pytest.raises(g4.G4Error):
+            g4.beam_workspace(*bad)
+
+
+def test_reorder_refusals(g4):
+    f = g4.load().g4_kv4_reorder
+    far = P + (1 << 20)
+
+    def call(caches=None, layers=None, g=2, w=4, pa=P, le=P, ti=P, to=far, stride=4, si=P, so=far):
+        cs = g4.kv4_caches(caches or [cache(g4), cache(g4, head_dim=512)])
+        return f(cs, len(cs) if layers is None else layers, g, w, pa, le, ti, to, stride, si, so, None)
+    for kw in BAD_CACHE:
+        assert call(caches=[cache(g4), cache(g4, **kw)]) == -1, kw
+    for kw in (dict(caches=[cache(g4), cache(g4, page_size=32)]), dict(caches=[cache(g4), cache(g4, num_pages=5)]),
+               dict(layers=0), dict(layers=65), dict(g=-1), dict(g=65537), dict(w=0), dict(w=33), dict(pa=None),
+               dict(le=None), dict(ti=None), dict(to=None), dict(si=None), dict(so=None), dict(to=P), dict(so=P),
+               dict(to=P + 4 * 4 * 8 - 4), dict(so=P + 4 * 8 - 4), dict(stride=0), dict(pa=P + 2)):
+        assert call(**kw) == -1, kw
+    assert call(g=0) == 0
+
+
+def test_reference_layout_is_a_bijection():
+    """Every nibble and scale of a record belongs to one token and dimension."""
+    rng = np.random.default_rng(0)
+    for hd in (64, 256):
+        c = ref.Cache(1, 16, 1, hd, fill=0)
+        seen = np.zeros(17 * hd, np.int64)
+        for t in range(16):
+            c.bytes[:] = 0
+            x = rng.standard_normal(hd) + 0.1
+            c.put(0, t, 0, x, x)
+            seen += c.bytes[0, 0, 0] != 0
+        assert (seen > 0).all() and (seen <= 2).all()
+
+
+def test_reference_rounding():
+    """Ties to even, exact next to a border, special groups."""
+    x = np.zeros((5, 64))
+    x[0, :4] = [7, 0.5, 1.5, -2.5]                     # scale 1: 0, 2, -2
+    x[1, :2] = [7, np.nextafter(np.float32(0.5), np.float32(1))]
+    x[2, 3] = np.inf
+    x[3, 5] = 2.0 ** -101
+    x[4, 0] = np.nan
+    c, s = ref.quantise(x)
+    assert c[0, :4].tolist() == [7, 0, 2, -2] and c[1, 1] == 1
+    assert np.isnan(s[2, 0]) and np.isnan(s[4, 0]) and s[3, 0] == 0 and not c[2:].any()
+
+
+def test_no_gpu_is_an_error(g4):
+    """Valid arguments without a GPU: an error code, no abort."""
+    torch = pytest.importorskip("torch")
+    if torch.cuda.is_available():
+        pytest.skip("has a GPU")
+    L = g4.load()
+    assert L.g4_kv4_write(cache(g4), batch(g4), 0, P, 256, P, 256, None) in (-1, -3)
