@@ -342,7 +342,9 @@ int kv4_check_cache(const g4_kv4_cache *c) {
 
 int kv4_view(const g4_kv4_cache *c, const g4_kv4_batch *b, Kv4View *v) {
     if (kv4_check_cache(c) != G4_OK || !b) return G4_ERR_INVALID;
-    if (b->n < 0 || b->n > 65536 || b->rows < 0 || b->rows > 1 << 22 || b->table_stride < 1) return G4_ERR_INVALID;
+    if (b->n < 0 || b->n > 65536 || b->rows < 0 || b->rows > 1 << 22 || b->table_stride < 1 ||
+        (int64_t)b->table_stride * c->page_size > 1 << 30)
+        return G4_ERR_INVALID;
     if (!b->offsets || !b->start_pos || !b->page_table || !aligned4(b->offsets) || !aligned4(b->start_pos) ||
         !aligned4(b->page_table))
         return G4_ERR_INVALID;

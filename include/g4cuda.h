@@ -162,7 +162,7 @@ typedef struct g4_kv4_batch {
     const int *offsets;       /* device, [n + 1], ascending */
     const int *start_pos;     /* device, [n] */
     const int *page_table;    /* device, [n][table_stride] */
-    int table_stride;
+    int table_stride;         /* 1.., table_stride * page_size <= 2^30 */
 } g4_kv4_batch;
 
 /* Bytes of one page, 0 for a geometry that is not supported. */

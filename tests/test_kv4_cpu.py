@@ -26,7 +26,8 @@ BAD_CACHE = [dict(pages=None), dict(pages=P + 8), dict(num_pages=0), dict(page_s
              dict(head_dim=0), dict(head_dim=1024)]
 BAD_BATCH = [dict(n=-1), dict(n=65537), dict(rows=-1), dict(rows=(1 << 22) + 1), dict(offsets=None),
              dict(start_pos=None), dict(page_table=None), dict(offsets=P + 2), dict(page_table=P + 1),
-             dict(table_stride=0)]
+             dict(table_stride=0),
+             dict(table_stride=(1 << 24) + 1)]
 
 
 def test_page_bytes(g4):
