@@ -18,9 +18,13 @@
 //                operands. The 8 is taken off in the accumulator's start value,
 //                -8 sum(q). q is scaled per row to 2^13..2^14 and, if fp32, split
 //                into high and low halves (22 bits).
-//   O^T = V^T P^T  bf16 (the scaled probabilities need its range): codes are
-//                (128 + n) - 136, exact; p vs is split into high and low bf16
-//                (16 bits).
+//   O^T = V^T P^T  bf16, whose range needs no common factor over the scales. A
+//                nibble is the bf16 subnormal n 2^-133 (16 n 2^-133 one nibble up);
+//                a packed add takes the 8 off, because the accumulator runs over all
+//                keys and an offset there would add up the truncations of the tensor
+//                core. p is 2^80 times too large to keep sums away from 2^-126: values
+//                up to 2^38 times a code are safe. p vs is split into high and low
+//                bf16 (16 bits) by packed FMAs on p's own halves.
 // Every warp streams its own records of 16 keys through a ring in shared memory
 // and keeps its own running maximum, sum and output; the warps meet once per
 // sequence and head. Work is counted in records over all (sequence, row tile, kv
@@ -34,28 +38,40 @@
 namespace {
 
 constexpr int kRows = 8;          // query rows of a tile (tokens x heads of one kv head)
-constexpr int kWarps = 8;
-constexpr int kThreads = kWarps * 32;
+constexpr int kStreams = 8;       // records in work at a time in one CTA
 constexpr int kSms = 148;
+constexpr int kJoinThreads = 256;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kSlack = 8.0f;                      // log2 of how far p may pass 1
+constexpr float kUp = 80.0f;                        // p is 2^80 times too large
+constexpr float kEven = 0x1p53f, kOdd = 0x1p49f;    // outputs: 2^133 / 2^80, 16 times less for odd dimensions
 
+// A record is worked on by kSplit warps, each for kDw dimensions of keys and
+// values: 512 dimensions take two, because the output of 8 rows x 512 in one
+// warp's registers leaves room for only 8 warps on an SM, too few to hide the
+// chain of a record (131072 keys: 32 us with one warp, see the figures below).
 template <int HD>
 struct Cfg {
-    static constexpr int G = HD / kKv4Group;
+    static constexpr int kSplit = HD == 512 ? 2 : 1;
+    static constexpr int kDw = HD / kSplit;
+    static constexpr int G = kDw / kKv4Group;                   // groups of a warp
+    static constexpr int kWarps = kStreams * kSplit;
+    static constexpr int kThreads = kWarps * 32;
     static constexpr int kRec = 17 * HD;
-    static constexpr int kStages = HD == 512 ? 3 : HD == 256 ? 3 : HD == 128 ? 4 : 6;
+    static constexpr int kStages = HD >= 256 ? 3 : HD == 128 ? 4 : 6;
     static constexpr int kOcc = HD == 512 ? 1 : 2;
     static constexpr int kCtas = kSms * kOcc;
-    static constexpr int kRing = kWarps * kStages * kRec;
-    static constexpr int kQ = G * 1024;                         // operands of the query tile (one half)
-    static constexpr int kPad = HD + 8;                         // row of the warps' outputs when they meet
+    static constexpr int kRing = kStreams * kStages * kRec;
+    static constexpr int kQ = HD / kKv4Group * 1024;            // operands of the query tile (one half)
+    static constexpr int kPad = kDw + 2;                        // row of a warp's output when the warps meet
     static constexpr int kSlot = 2 * kRows + kRows * HD;        // floats of one partial result
-    static_assert(kStages * kRec >= kRows * kPad * 4, "a warp's ring holds its output tile");
+    static_assert(kStages * kRec >= kSplit * kRows * kPad * 4, "a stream's ring holds its output tile");
 };
 
 struct AttnP {
     Kv4View c;
-    int type, group;              // query heads per kv head
+    int type;
+    unsigned group;               // query heads per kv head
     const void *q;
     void *out;
     long long q_stride, out_stride;
@@ -64,12 +80,13 @@ struct AttnP {
     float *slots;                 // partial results, two per CTA
 };
 
-G4_DEV void cp16(uint32_t dst, const void *src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+G4_DEV void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
+    asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                     smem_u32(dst)),
+                 "l"(src), "r"(bytes), "r"(smem_u32(bar))
+                 : "memory");
 }
-G4_DEV void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-G4_DEV void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+G4_DEV void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 G4_DEV void mma_h(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -99,13 +116,24 @@ G4_DEV void transpose2(float &a, float &b) {
     a = __uint_as_float(__byte_perm(lo, hi, 0x5410));
     b = __uint_as_float(__byte_perm(lo, hi, 0x7632));
 }
-// nibbles at bits [s, s + 4) of both halves -> the codes as bf16
-G4_DEV uint32_t code_b(uint32_t x, int s) {
-    const uint32_t w = ((x >> s) & 0x000f000fu) | 0x43004300u;      // 128 + n
+G4_DEV uint32_t add_b(uint32_t a, uint32_t b) {
     uint32_t y;
-    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(w), "r"(0x43084308u));
+    asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
     return y;
 }
+G4_DEV uint32_t mul_b(uint32_t a, uint32_t b) {
+    uint32_t y;
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
+    return y;
+}
+G4_DEV uint32_t fma_b(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t y;
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(y) : "r"(a), "r"(b), "r"(c));
+    return y;
+}
+// Codes of the low nibble of each half's low byte as bf16 c 2^-133, of the high nibble as 16 c 2^-133
+G4_DEV uint32_t code_lo(uint32_t x) { return add_b(x & 0x000f000fu, 0x80088008u); }
+G4_DEV uint32_t code_hi(uint32_t x) { return add_b(x & 0x00f000f0u, 0x80808080u); }
 G4_DEV uint32_t pack_b(float lo, float hi) {
     uint32_t y;
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
@@ -129,10 +157,34 @@ G4_DEV void store8(void *p, int type, long long i, const float (&x)[8]) {
     else Kv4Vec<__half>::store((__half *)p + i, x);
 }
 
+G4_DEV void store2(void *p, int type, long long i, float x, float y) {
+    if (type == G4_TYPE_F32) *reinterpret_cast<float2 *>((float *)p + i) = make_float2(x, y);
+    else *reinterpret_cast<uint32_t *>((uint16_t *)p + i) = type == G4_TYPE_BF16 ? pack_b(x, y) : pack_h(x, y);
+}
+
+// N bf16 scales, and one of a pair as fp32
+template <int N>
+G4_DEV void load_scales(const void *p, uint32_t (&w)[(N + 1) / 2]) {
+    if constexpr (N == 4) {
+        const uint2 x = *reinterpret_cast<const uint2 *>(p);
+        w[0] = x.x;
+        w[1] = x.y;
+    } else if constexpr (N == 2) w[0] = *reinterpret_cast<const uint32_t *>(p);
+    else w[0] = *reinterpret_cast<const uint16_t *>(p);
+}
+G4_DEV float half_of(uint32_t w, int i) { return __uint_as_float(i ? w & 0xffff0000u : w << 16); }
+
+constexpr int kItemCost = 16;
+constexpr int kSeqs = 32;         // sequences described in shared memory at a time
+
 // ---- the schedule -------------------------------------------------------------
 // Sequence b: its rows in tiles of kRows, each tile x kv head an item of `recs`
 // records (those that the sequence's rows see between them; a tile skips what
-// its own rows do not see; at least 1, so that empty rows are written).
+// its own rows do not see; at least 1, so that empty rows are written). An item
+// counts kItemCost + recs units of work: its queries, the meeting of its warps and
+// its output take about as long as kItemCost records (a 64-sequence step with
+// contexts of 128 to 8704: the CTAs that got only short sequences took 60 us, the
+// others 28, when items counted their records alone).
 struct Seq {
     int row0, q, tiles, recs, rec0;
     long long pos0;
@@ -143,21 +195,19 @@ G4_DEV Seq seq_of(const AttnP &p, int b) {
     s.row0 = kv4_offset(p.c, b);
     s.q = max(kv4_offset(p.c, b + 1) - s.row0, 0);
     s.pos0 = p.c.start_pos[b];
-    s.tiles = (int)(((long long)s.q * p.group + kRows - 1) / kRows);
+    s.tiles = (s.q * p.group + kRows - 1) / kRows;            // q <= 2^22, group <= 64
     const long long lo = p.window ? max(s.pos0 - p.window + 1, 0ll) : 0;
     const long long hi = min(s.pos0 + s.q - 1, ((long long)p.c.table_stride << p.c.page_shift) - 1);
     s.rec0 = (int)(lo >> 4);
     s.recs = hi < lo ? 1 : (int)((hi >> 4) - (lo >> 4)) + 1;
     return s;
 }
-G4_DEV long long work_of(const AttnP &p, const Seq &s) { return (long long)s.tiles * p.c.kv_heads * s.recs; }
+G4_DEV long long work_of(const AttnP &p, const Seq &s) {
+    return (long long)s.tiles * p.c.kv_heads * (s.recs + kItemCost);
+}
 
-// Total work, and where unit `w` of it lies: sequence and offset in its work.
-// Every thread of a block of N calls it; `s` is shared memory.
-struct Where {
-    long long total, off;
-    int seq;
-};
+// Total work, and the sequence in which unit `w` of it lies with w's offset in
+// that sequence's work. Every thread of a block of N calls them.
 template <int N>
 struct Scan {
     long long warp[N / 32], off;
@@ -177,6 +227,7 @@ G4_DEV long long scan_total(const AttnP &p, Scan<N> &s, int per, long long &befo
     if (lane == 31) s.warp[tid >> 5] = inc;
     __syncthreads();
     long long total = 0, base = 0;
+#pragma unroll
     for (int i = 0; i < N / 32; i++) {
         if (i < (tid >> 5)) base += s.warp[i];
         total += s.warp[i];
@@ -185,8 +236,7 @@ G4_DEV long long scan_total(const AttnP &p, Scan<N> &s, int per, long long &befo
     return total;
 }
 template <int N>
-G4_DEV Where find_work(const AttnP &p, Scan<N> &s, int per, long long total, long long before, long long mine,
-                       long long w) {
+G4_DEV void find_work(const AttnP &p, Scan<N> &s, int per, long long before, long long mine, long long w) {
     if (w >= before && w < before + mine) {
         long long at = before;
         int b = threadIdx.x * per;
@@ -199,148 +249,233 @@ G4_DEV Where find_work(const AttnP &p, Scan<N> &s, int per, long long total, lon
         s.off = w - at;
     }
     __syncthreads();
-    return {total, s.off, s.seq};
 }
-G4_DEV long long share_of(long long total, int ctas) { return max((total + ctas - 1) / ctas, (long long)kWarps); }
+G4_DEV long long share_of(long long total, int ctas) {
+    // a 64-bit division costs as much as a load; most totals fit 32 bits
+    const unsigned long long t = (unsigned long long)total + ctas - 1;
+    const long long s = t >> 32 ? (long long)(t / ctas) : (long long)((unsigned)t / (unsigned)ctas);
+    return max(s, (long long)kItemCost + kStreams);      // at least a round of records for who starts an item
+}
+// x / y and x % y for 0 <= x, 0 < y < 2^31
+G4_DEV void divide(long long x, int y, int &q, int &r) {
+    if ((unsigned long long)x >> 32) {
+        q = (int)(x / y);
+        r = (int)(x - (long long)q * y);
+    } else {
+        q = (int)((unsigned)x / (unsigned)y);
+        r = (int)((unsigned)x - (unsigned)q * (unsigned)y);
+    }
+}
 
 // ---- the streaming kernel -------------------------------------------------------
+// What a CTA does of one item: records [ra, rb) of sequence b for kv head h and
+// the rows [tile * kRows, + valid) of its group.
+struct Item {
+    int b, h, tile, valid, row0;
+    int ra, rb;
+    int all0, all1;            // every row sees the keys all0..all1
+    long long pos0;
+    int whole, starts, none;   // none: the CTA has no more work
+};
+
+// The CTA's way through its work, kept in shared memory by its last warp: the
+// sequence (a run of kSeqs of them described at a time), the item of it and the
+// unit of that where the next item starts.
+struct Walk {
+    long long left;
+    int b, cached, item, unit;
+    Seq seqs[kSeqs];
+};
+
+// The next item, by one whole warp.
+G4_DEV void next_item(const AttnP &p, Walk &w, Item &out) {
+    const int lane = threadIdx.x & 31, kvh = p.c.kv_heads;
+    if (w.left <= 0) {
+        if (lane == 0) out.none = 1;
+        return;
+    }
+    int b = w.b, item = w.item;
+    for (;; b++, item = 0) {
+        if (b >= w.cached + kSeqs) {
+            __syncwarp();
+            if (b + lane < p.c.n) w.seqs[lane] = seq_of(p, b + lane);
+            if (lane == 0) w.cached = b;
+            __syncwarp();
+        }
+        if (item < w.seqs[b - w.cached].tiles * kvh) break;         // an empty sequence has no items
+    }
+    __syncwarp();
+    if (lane) return;
+    const int cap = p.c.table_stride << p.c.page_shift;              // <= 2^30
+    const Seq s = w.seqs[b - w.cached];
+    // units [u0, u1) of the item, of which the first kItemCost are no records: who
+    // holds only such leaves the item to the next CTA
+    const int u0 = w.unit, u1 = (int)min((long long)s.recs + kItemCost, u0 + w.left);
+    const int r0 = max(u0 - kItemCost, 0), r1 = u1 - kItemCost;
+    w.left -= u1 - u0;
+    w.b = b;
+    w.item = item + 1;
+    w.unit = 0;
+    if (r1 <= 0) {             // only at the end of the CTA's work; nothing else of `out` is set
+        out.none = 1;
+        return;
+    }
+    Item it;
+    it.none = 0;
+    it.b = b;
+    it.tile = (unsigned)item / (unsigned)kvh;
+    it.h = item - it.tile * kvh;
+    it.whole = r0 == 0 && r1 == s.recs;
+    it.starts = r0 == 0;
+    it.row0 = s.row0;
+    it.pos0 = s.pos0;
+    // rows are (token, head of the group), token-major
+    const unsigned first = it.tile * kRows;
+    it.valid = min((int)(s.q * p.group - first), kRows);
+    const long long pos_first = s.pos0 + first / p.group, pos_last = s.pos0 + (first + it.valid - 1) / p.group;
+    const int see0 = p.window ? (int)min(max(pos_first - p.window + 1, 0ll), (long long)cap) : 0;
+    const int see1 = (int)max(min(pos_last, (long long)cap - 1), -1ll);              // some row sees [see0, see1]
+    it.all0 = p.window ? (int)min(max(pos_last - p.window + 1, 0ll), (long long)cap) : 0;
+    it.all1 = (int)max(min(pos_first, (long long)cap - 1), -1ll);
+    it.ra = max(s.rec0 + r0, see0 >> 4);
+    it.rb = see1 < see0 ? it.ra : min(s.rec0 + r1, (see1 >> 4) + 1);
+    out = it;
+}
+
 template <int HD, bool HILO>
-__global__ void __launch_bounds__(kThreads, Cfg<HD>::kOcc) k_kv4_attn(const __grid_constant__ AttnP p) {
+__global__ void __launch_bounds__(Cfg<HD>::kThreads, Cfg<HD>::kOcc) k_kv4_attn(const __grid_constant__ AttnP p) {
     using C = Cfg<HD>;
-    constexpr int G = C::G, REC = C::kRec, ST = C::kStages;
+    constexpr int G = C::G, REC = C::kRec, ST = C::kStages, DW = C::kDw, HG = HD / kKv4Group;
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t *ring = smem;
-    uint4 *qhi = reinterpret_cast<uint4 *>(smem + C::kRing);            // [G][2][32] (lane's operands of two steps)
+    uint4 *qhi = reinterpret_cast<uint4 *>(smem + C::kRing);            // [HD / 64][2][32] (lane's operands of two steps)
     uint4 *qlo = qhi + C::kQ / 16;
-    float *qoff = reinterpret_cast<float *>(smem + C::kRing + (HILO ? 2 : 1) * C::kQ);   // [G][8]: -8 sum q
-    __shared__ Scan<kThreads> scan;
-    __shared__ float row_scale[kRows], sm_m[kWarps][kRows], sm_l[kWarps][kRows];
-    __shared__ int sm_ok[kWarps][8];
+    float *qoff = reinterpret_cast<float *>(smem + C::kRing + (HILO ? 2 : 1) * C::kQ);   // [HD / 64][8]: -8 sum q
+    __shared__ Scan<C::kThreads> scan;
+    __shared__ Walk walk;
+    __shared__ Item items[2];
+    __shared__ float row_scale[kRows], row_max[C::kWarps], sm_m[kStreams][kRows], sm_l[kStreams][kRows];
+    __shared__ uint64_t full[kStreams][ST];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int group = p.group, kvh = p.c.kv_heads;
-    const long long cap = (long long)p.c.table_stride << p.c.page_shift;
+    const int stream = warp / C::kSplit, part = warp % C::kSplit;       // this warp: groups [part * G, + G)
+    const unsigned group = p.group;
 
-    const int per = (p.c.n + kThreads - 1) / kThreads;
+    if (tid < kStreams * ST) mbar_init(&full[0][0] + tid, 1);
+    mbar_fence_init();
+    const int per = (p.c.n + C::kThreads - 1) / C::kThreads;
     long long before, mine;
     const long long total = scan_total(p, scan, per, before, mine);
     const long long share = share_of(total, C::kCtas);
-    const long long w0 = blockIdx.x * share, w1 = min(total, w0 + share);
-    if (w0 >= w1) return;
-    const Where at = find_work(p, scan, per, total, before, mine, w0);
-    int b = at.seq;
-    long long off = at.off;
-    uint8_t *my_ring = ring + warp * (ST * REC);
-
-    for (long long w = w0; w < w1;) {
-        const Seq s = seq_of(p, b);
-        const long long work = work_of(p, s);
-        if (off >= work) {          // next sequence (empty ones have no work)
-            off -= work;
-            b++;
-            continue;
+    const long long w0 = blockIdx.x * share;
+    griddep_launch();
+    if (w0 >= total) return;
+    find_work(p, scan, per, before, mine, w0);
+    if (warp == C::kWarps - 1) {
+        if (lane == 0) {
+            walk.left = min(total - w0, share);
+            walk.b = scan.seq;
+            walk.cached = -kSeqs;
+            divide(scan.off, seq_of(p, scan.seq).recs + kItemCost, walk.item, walk.unit);
         }
-        const int item = (int)(off / s.recs), r0 = (int)(off % s.recs);
-        const int r1 = (int)min((long long)s.recs, r0 + (w1 - w));
-        const int tile = item / kvh, h = item % kvh;
-        const bool whole = r0 == 0 && r1 == s.recs;
-        const bool starts = r0 == 0;
-        w += r1 - r0;
-        off += r1 - r0;
-
-        // what the tile's rows see: rows are (token, head of the group), token-major
-        const long long rows_left = (long long)s.q * group - (long long)tile * kRows;
-        const int valid = (int)min(rows_left, (long long)kRows);
-        const long long tok0 = (long long)tile * kRows / group, tok1 = ((long long)tile * kRows + valid - 1) / group;
-        const long long pos_first = s.pos0 + tok0, pos_last = s.pos0 + tok1;
-        const long long see0 = p.window ? max(pos_first - p.window + 1, 0ll) : 0;       // any row sees [see0, see1]
-        const long long see1 = min(pos_last, cap - 1);
-        const long long all0 = p.window ? max(pos_last - p.window + 1, 0ll) : 0;        // every row sees [all0, pos_first]
-        const int ra = max(s.rec0 + r0, (int)(see0 >> 4));
-        const int rb = see1 < see0 ? ra : min(s.rec0 + r1, (int)(see1 >> 4) + 1);
-        const int nmine = max(0, (rb - ra - warp + kWarps - 1) / kWarps);               // records of this warp
-        // this lane's row g
-        const long long idx = (long long)tile * kRows + g;
-        const long long row_pos = s.pos0 + idx / group;
-        const int my_hi = g < valid ? (int)max(min(row_pos, cap - 1), -1ll) : -1;
-        const int my_lo = p.window ? (int)min(max(row_pos - p.window + 1, 0ll), cap) : 0;
-
-        // addresses of the next 32 of this warp's records, one per lane
-        unsigned long long addr = 0;
-        auto lookup = [&](int k0) {
-            const int k = k0 + lane;
-            addr = 0;
-            if (k < nmine)
-                addr = (unsigned long long)kv4_record(p.c, b, (long long)(ra + warp + k * kWarps) * 16, h);
-        };
-        auto issue = [&](int k) {
-            if (k < nmine) {
-                if ((k & 31) == 0) lookup(k);
-                const uint8_t *src = (const uint8_t *)__shfl_sync(0xffffffffu, addr, k & 31);
-                if (lane == 0) sm_ok[warp][k % ST] = src != nullptr;
-                if (src) {
-                    const uint32_t dst = smem_u32(my_ring + (k % ST) * REC);
+        __syncwarp();
+        next_item(p, walk, items[0]);
+    }
+    __syncthreads();
+    uint8_t *my_ring = ring + stream * (ST * REC);
+    uint32_t phase = 0;                                                 // of the stream's stages, one bit each
+    // addresses of records k0 .. k0 + 31 of this stream, one per lane
+    auto lookup = [&](const Item &it, int k0) -> unsigned long long {
+        const int rec = it.ra + stream + (k0 + lane) * kStreams;
+        return rec < it.rb ? (unsigned long long)kv4_record(p.c, it.b, (long long)rec * 16, it.h) : 0;
+    };
+    // 8 dimensions of a query row per thread
+    const int qr = tid / (HD / 8), qc = tid % (HD / 8);
+    auto load_q = [&](const Item &it, float (&x)[8]) {
 #pragma unroll
-                    for (int i = 0; i < (REC / 16 + 31) / 32; i++)
-                        if (i * 32 + lane < REC / 16) cp16(dst + (i * 32 + lane) * 16, src + (i * 32 + lane) * 16);
-                }
+        for (int i = 0; i < 8; i++) x[i] = 0.0f;
+        if (qr < it.valid) {
+            const unsigned ri = it.tile * kRows + qr, tok = ri / group;
+            load8(p.q, p.type, (it.row0 + (long long)tok) * p.q_stride + (long long)(it.h * group + (ri - tok * group)) * HD + qc * 8, x);
+        }
+    };
+
+    unsigned long long addr = 0;
+    float qx[8];
+    if (!items[0].none) {
+        addr = lookup(items[0], 0);
+        load_q(items[0], qx);
+    }
+    for (int cur = 0; !items[cur].none; cur ^= 1) {
+        const Item &it = items[cur];
+        const int ra = it.ra, all0 = it.all0, all1 = it.all1;
+        const int nmine = max(0, (it.rb - ra - stream + kStreams - 1) / kStreams);    // records of this stream
+        uint32_t there = 0;                 // stages that hold a record (not of a missing page)
+        auto issue = [&](int k) {
+            if (k >= nmine) return;
+            if ((k & 31) == 0 && k) addr = lookup(it, k);
+            const uint8_t *src = (const uint8_t *)__shfl_sync(0xffffffffu, addr, k & 31);
+            const int st = k % ST;
+            there = src ? there | 1u << st : there & ~(1u << st);
+            if (src && part == 0 && lane == 0) {
+                mbar_arrive_expect_tx(&full[stream][st], REC);
+                bulk_load(my_ring + st * REC, src, REC, &full[stream][st]);
             }
-            cp_commit();
         };
         for (int k = 0; k < ST - 1; k++) issue(k);
+        if (warp == C::kWarps - 1) next_item(p, walk, items[cur ^ 1]);
 
-        // query operands: warp r prepares row r, 8 dimensions a lane
-        __syncthreads();            // the previous item's operands are no longer read
+        // query operands
         {
-            const int r = warp;
-            const long long ri = (long long)tile * kRows + r;
-            const long long at_q = (s.row0 + ri / group) * p.q_stride + (long long)(h * group + ri % group) * HD;
-            constexpr int NC = (HD / 8 + 31) / 32;
-            float x[NC][8], mx = 0.0f;
+            float mx = 0.0f;
 #pragma unroll
-            for (int c = 0; c < NC; c++) {
+            for (int i = 0; i < 8; i++) mx = fmaxf(mx, fabsf(qx[i]));
 #pragma unroll
-                for (int i = 0; i < 8; i++) x[c][i] = 0.0f;
-                if (r < valid && c * 32 + lane < HD / 8) load8(p.q, p.type, at_q + (c * 32 + lane) * 8, x[c]);
-#pragma unroll
-                for (int i = 0; i < 8; i++) mx = fmaxf(mx, fabsf(x[c][i]));
+            for (int o = 1; o < min(32, HD / 8); o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+            if constexpr (HD / 8 > 32) {
+                if (lane == 0) row_max[warp] = mx;
+                __syncthreads();
+                mx = fmaxf(mx, row_max[warp ^ 1]);
             }
-            mx = warp_max(mx);
             // exact power of two that brings the row's largest |q| to 2^13..2^14
             const int e = min(max((int)(__float_as_uint(mx) >> 23) - 127, -100), 115);
             const float up = __uint_as_float((uint32_t)(127 + 13 - e) << 23);
-            if (lane == 0) row_scale[r] = p.scale * kLog2e * __uint_as_float((uint32_t)(127 + 24 - 13 + e) << 23);
+            // 8 dimensions: group qc / 8, t = qc / 2 % 4, half qc % 2; steps 2 half + i take
+            // dimensions 2i, 2i+4 and, a nibble up, 2i+1, 2i+5
+            float rep = 0.0f;
+            uint32_t hi[4], lo[4];
 #pragma unroll
-            for (int c = 0; c < NC; c++) {
-                const int ch = c * 32 + lane;             // chunk of 8 dimensions: group ch / 8, t = ch / 2 % 4, half ch % 2
-                float rep = 0.0f;
-                uint32_t hi[4], lo[4];
-#pragma unroll
-                for (int i = 0; i < 2; i++) {             // steps 2 half + i: dimensions 2i, 2i+4 and (a nibble up) 2i+1, 2i+5
-                    const float y[4] = {x[c][2 * i] * up, x[c][2 * i + 4] * up, x[c][2 * i + 1] * up * 0.0625f,
-                                        x[c][2 * i + 5] * up * 0.0625f};
-                    hi[2 * i] = pack_h(y[0], y[1]);
-                    hi[2 * i + 1] = pack_h(y[2], y[3]);
-                    float2 f0 = unpack_h(hi[2 * i]), f1 = unpack_h(hi[2 * i + 1]);
+            for (int i = 0; i < 2; i++) {
+                const float y[4] = {qx[2 * i] * up, qx[2 * i + 4] * up, qx[2 * i + 1] * up * 0.0625f,
+                                    qx[2 * i + 5] * up * 0.0625f};
+                hi[2 * i] = pack_h(y[0], y[1]);
+                hi[2 * i + 1] = pack_h(y[2], y[3]);
+                float2 f0 = unpack_h(hi[2 * i]), f1 = unpack_h(hi[2 * i + 1]);
+                rep += f0.x + f0.y + 16.0f * (f1.x + f1.y);
+                if (HILO) {
+                    lo[2 * i] = pack_h(y[0] - f0.x, y[1] - f0.y);
+                    lo[2 * i + 1] = pack_h(y[2] - f1.x, y[3] - f1.y);
+                    f0 = unpack_h(lo[2 * i]);
+                    f1 = unpack_h(lo[2 * i + 1]);
                     rep += f0.x + f0.y + 16.0f * (f1.x + f1.y);
-                    if (HILO) {
-                        lo[2 * i] = pack_h(y[0] - f0.x, y[1] - f0.y);
-                        lo[2 * i + 1] = pack_h(y[2] - f1.x, y[3] - f1.y);
-                        f0 = unpack_h(lo[2 * i]);
-                        f1 = unpack_h(lo[2 * i + 1]);
-                        rep += f0.x + f0.y + 16.0f * (f1.x + f1.y);
-                    }
                 }
+            }
 #pragma unroll
-                for (int o = 1; o < 8; o <<= 1) rep += __shfl_xor_sync(0xffffffffu, rep, o);
-                if (ch < HD / 8) {
-                    const int to = ((ch >> 3) * 2 + (ch & 1)) * 32 + r * 4 + (ch >> 1 & 3);
-                    qhi[to] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                    if (HILO) qlo[to] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                    if ((ch & 7) == 0) qoff[(ch >> 3) * 8 + r] = -8.0f * 0x1p-24f * rep;
-                }
+            for (int o = 1; o < 8; o <<= 1) rep += __shfl_xor_sync(0xffffffffu, rep, o);
+            if (qr < kRows) {
+                if (qc == 0)
+                    row_scale[qr] = p.scale * kLog2e * __uint_as_float((uint32_t)(127 + 24 - 13 + e) << 23);
+                const int to = ((qc >> 3) * 2 + (qc & 1)) * 32 + qr * 4 + (qc >> 1 & 3);
+                qhi[to] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                if (HILO) qlo[to] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                if ((qc & 7) == 0) qoff[(qc >> 3) * 8 + qr] = -8.0f * 0x1p-24f * rep;
             }
         }
         __syncthreads();
+        // this lane's row g sees the keys my_lo..my_hi
+        const long long row_pos = it.pos0 + (it.tile * kRows + g) / group;
+        const int cap = p.c.table_stride << p.c.page_shift;
+        const int my_hi = g < it.valid ? (int)max(min(row_pos, (long long)cap - 1), -1ll) : -1;
+        const int my_lo = p.window ? (int)min(max(row_pos - p.window + 1, 0ll), (long long)cap) : 0;
 
         float o[G][4][4];
 #pragma unroll
@@ -352,28 +487,42 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kOcc) k_kv4_attn(const __gr
         float m = -INFINITY, l = 0.0f;
         const float rs0 = row_scale[2 * t], rs1 = row_scale[2 * t + 1];
 
+        bool lost = false;                                    // a copy that never came
         for (int k = 0; k < nmine; k++) {
-            cp_wait<ST - 2>();
-            __syncwarp();
-            issue(k + ST - 1);
-            if (!sm_ok[warp][k % ST]) continue;           // no page: no keys
-            const uint8_t *rec = my_ring + (k % ST) * REC;
-            const int key0 = (ra + warp + k * kWarps) * 16;
+            const int st = k % ST;
+            if (C::kSplit == 1) {
+                __syncwarp();
+                issue(k + ST - 1);
+            }
+            if (!(there >> st & 1)) {                         // no page: no keys (for all warps of the record)
+                if (C::kSplit > 1) {
+                    bar_sync(1 + stream, 32 * C::kSplit);
+                    issue(k + ST - 1);
+                }
+                continue;
+            }
+            if (!mbar_wait(&full[stream][st], phase >> st & 1, nullptr, 0)) lost = true;
+            phase ^= 1u << st;
+            uint8_t *rec = my_ring + st * REC;
+            const int key0 = (ra + stream + k * kStreams) * 16;
 
             // ---- scores: lane holds keys g, g + 8 x rows 2t, 2t + 1 ----
             float sc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            const uint16_t *ks = reinterpret_cast<const uint16_t *>(rec + 16 * HD) + g * G;
+            uint32_t k0s[(G + 1) / 2], k1s[(G + 1) / 2];      // scales of keys g and g + 8
+            load_scales<G>(rec + 16 * HD + g * (2 * HG) + part * (2 * G), k0s);
+            load_scales<G>(rec + 16 * HD + (g + 8) * (2 * HG) + part * (2 * G), k1s);
 #pragma unroll
             for (int gr = 0; gr < G; gr++) {
-                const uint4 kc = *reinterpret_cast<const uint4 *>(rec + gr * 512 + lane * 16);
-                const float2 q0 = *reinterpret_cast<const float2 *>(qoff + gr * 8 + 2 * t);
+                const uint4 kc = *reinterpret_cast<const uint4 *>(rec + (part * G + gr) * 512 + lane * 16);
+                const float2 q0 = *reinterpret_cast<const float2 *>(qoff + (part * G + gr) * 8 + 2 * t);
                 float d[4] = {q0.x, q0.y, q0.x, q0.y};
 #pragma unroll
                 for (int half = 0; half < 2; half++) {
                     uint32_t x = half ? kc.y : kc.x, z = half ? kc.w : kc.z;
-                    const uint4 bh = qhi[(gr * 2 + half) * 32 + lane];
+                    const int qi = ((part * G + gr) * 2 + half) * 32 + lane;
+                    const uint4 bh = qhi[qi];
                     uint4 bl;
-                    if (HILO) bl = qlo[(gr * 2 + half) * 32 + lane];
+                    if (HILO) bl = qlo[qi];
                     const uint32_t a0 = x & 0x000f000fu, a1 = z & 0x000f000fu, a2 = x & 0x00f000f0u,
                                    a3 = z & 0x00f000f0u;
                     mma_h(d, a0, a1, a2, a3, bh.x, bh.y);
@@ -385,11 +534,27 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kOcc) k_kv4_attn(const __gr
                     mma_h(d, a4, a5, a6, a7, bh.z, bh.w);
                     if (HILO) mma_h(d, a4, a5, a6, a7, bl.z, bl.w);
                 }
-                const float k0 = bf16_bits_f(ks[gr]), k1 = bf16_bits_f(ks[8 * G + gr]);
+                const float k0 = half_of(k0s[gr / 2], gr & 1), k1 = half_of(k1s[gr / 2], gr & 1);
                 sc[0] = fmaf(d[0], k0, sc[0]);
                 sc[1] = fmaf(d[1], k0, sc[1]);
                 sc[2] = fmaf(d[2], k1, sc[2]);
                 sc[3] = fmaf(d[3], k1, sc[3]);
+            }
+            if constexpr (C::kSplit > 1) {
+                // The other warp's groups: both add in the same order. A warp leaves its
+                // scores where its K codes were; the next copy into that stage is issued
+                // behind the barrier of the next record, when they have been read.
+                __syncwarp();
+                float4 *x4 = reinterpret_cast<float4 *>(rec) + lane;
+                x4[part * (8 * DW / 16)] = make_float4(sc[0], sc[1], sc[2], sc[3]);
+                fence_async();
+                bar_sync(1 + stream, 32 * C::kSplit);
+                issue(k + ST - 1);
+                const float4 x = x4[0], y = x4[8 * DW / 16];
+                sc[0] = x.x + y.x;
+                sc[1] = x.y + y.y;
+                sc[2] = x.z + y.z;
+                sc[3] = x.w + y.w;
             }
             sc[0] *= rs0;
             sc[1] *= rs1;
@@ -398,21 +563,25 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kOcc) k_kv4_attn(const __gr
             // ---- row g, keys 2t, 2t + 1, 2t + 8, 2t + 9 ----
             transpose2(sc[0], sc[1]);
             transpose2(sc[2], sc[3]);
-            const bool edge = key0 < all0 || key0 + 15 > pos_first;
-            bool see[4];
+            const bool edge = key0 < all0 || key0 + 15 > all1;
+            uint32_t see01 = 0, see23 = 0;
             if (edge) {
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const int key = key0 + 2 * t + (i & 1) + 8 * (i >> 1);
-                    see[i] = key >= my_lo && key <= my_hi;
-                    if (!see[i]) sc[i] = -INFINITY;
+                    const bool see = key >= my_lo && key <= my_hi;
+                    if (!see) sc[i] = -INFINITY;
+                    else if (i < 2) see01 |= 0xffffu << (16 * (i & 1));
+                    else see23 |= 0xffffu << (16 * (i & 1));
                 }
             }
             float mx = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            if (__any_sync(0xffffffffu, mx > m)) {
-                const float mn = fmaxf(m, mx);
+            // The reference m follows the maximum when that is kSlack above it: p stays
+            // below 2^kSlack, and the outputs are rescaled a few times per sequence.
+            if (__any_sync(0xffffffffu, mx > m + kSlack)) {
+                const float mn = mx > m + kSlack ? mx : m;
                 const float al = mn == -INFINITY ? 1.0f : ex2(m - mn);
                 m = mn;
                 l *= al;
@@ -427,154 +596,211 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kOcc) k_kv4_attn(const __gr
                         o[i][j][3] *= al1;
                     }
             }
-            const float mref = m == -INFINITY ? 0.0f : m;
+            const float mref = (m == -INFINITY ? 0.0f : m) - kUp;
             float pr[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) pr[i] = ex2(sc[i] - mref);
             l += (pr[0] + pr[1]) + (pr[2] + pr[3]);
+            // p as high and low bf16
+            const uint32_t ph0 = pack_b(pr[0], pr[1]), ph1 = pack_b(pr[2], pr[3]);
+            const uint32_t pl0 = pack_b(pr[0] - half_of(ph0, 0), pr[1] - half_of(ph0, 1));
+            const uint32_t pl1 = pack_b(pr[2] - half_of(ph1, 0), pr[3] - half_of(ph1, 1));
 
             // ---- output: lane holds dimensions 8g + 2j, + 1 of each group x rows 2t, 2t + 1 ----
-            const uint2 *vsp = reinterpret_cast<const uint2 *>(rec + 16 * HD + 32 * G) + t;
+            const uint2 *vsp = reinterpret_cast<const uint2 *>(rec + 16 * HD + 32 * HG + part * (32 * G)) + t;
 #pragma unroll
             for (int gr = 0; gr < G; gr++) {
-                const uint4 vc = *reinterpret_cast<const uint4 *>(rec + 8 * HD + gr * 512 + lane * 16);
-                const uint2 vs = vsp[gr * 4];
-                float pv[4] = {pr[0] * __uint_as_float(vs.x << 16), pr[1] * __uint_as_float(vs.x & 0xffff0000u),
-                               pr[2] * __uint_as_float(vs.y << 16), pr[3] * __uint_as_float(vs.y & 0xffff0000u)};
-                if (edge) {
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        if (!see[i]) pv[i] = 0.0f;        // the scale of a token that is not there may be anything
+                const uint4 vc = *reinterpret_cast<const uint4 *>(rec + 8 * HD + (part * G + gr) * 512 + lane * 16);
+                uint2 vs = vsp[gr * 4];
+                if (edge) {                               // the scale of a token that is not seen may be anything
+                    vs.x &= see01;
+                    vs.y &= see23;
                 }
-                const uint32_t h0 = pack_b(pv[0], pv[1]), h1 = pack_b(pv[2], pv[3]);
-                const uint32_t l0 = pack_b(pv[0] - __uint_as_float(h0 << 16), pv[1] - __uint_as_float(h0 & 0xffff0000u));
-                const uint32_t l1 = pack_b(pv[2] - __uint_as_float(h1 << 16), pv[3] - __uint_as_float(h1 & 0xffff0000u));
+                // p vs = h + l: h the rounded product of p's high half, l what it lost and the low half's product
+                const uint32_t h0 = mul_b(ph0, vs.x), h1 = mul_b(ph1, vs.y);
+                const uint32_t l0 = fma_b(pl0, vs.x, fma_b(ph0, vs.x, h0 ^ 0x80008000u));
+                const uint32_t l1 = fma_b(pl1, vs.y, fma_b(ph1, vs.y, h1 ^ 0x80008000u));
 #pragma unroll
                 for (int half = 0; half < 2; half++) {
-                    const uint32_t ab = __byte_perm(vc.x, vc.y, half ? 0x7632 : 0x5410);
-                    const uint32_t cd = __byte_perm(vc.z, vc.w, half ? 0x7632 : 0x5410);
+                    uint32_t ab = __byte_perm(vc.x, vc.y, half ? 0x7632 : 0x5410);
+                    uint32_t cd = __byte_perm(vc.z, vc.w, half ? 0x7632 : 0x5410);
 #pragma unroll
                     for (int i = 0; i < 2; i++) {
-                        const uint32_t a0 = code_b(ab, 8 * i), a1 = code_b(ab, 8 * i + 4), a2 = code_b(cd, 8 * i),
-                                       a3 = code_b(cd, 8 * i + 4);
+                        const uint32_t a0 = code_lo(ab), a1 = code_hi(ab), a2 = code_lo(cd), a3 = code_hi(cd);
                         mma_b(o[gr][2 * half + i], a0, a1, a2, a3, h0, h1);
                         mma_b(o[gr][2 * half + i], a0, a1, a2, a3, l0, l1);
+                        ab >>= 8;
+                        cd >>= 8;
                     }
                 }
             }
         }
-        cp_wait<0>();
-        __syncwarp();
+        if (lost) l = NAN;
 
-        // ---- the warps meet ----
+        // ---- the warps meet; the next item's addresses and queries are on their way ----
+        if (!items[cur ^ 1].none) {
+            addr = lookup(items[cur ^ 1], 0);
+            load_q(items[cur ^ 1], qx);
+        }
         l += __shfl_xor_sync(0xffffffffu, l, 1);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
-        if (t == 0) { sm_m[warp][g] = m; sm_l[warp][g] = l; }
-        float *ow = reinterpret_cast<float *>(my_ring);
+        l *= 0x1p-80f;
+        if (t == 0 && part == 0) { sm_m[stream][g] = m; sm_l[stream][g] = l; }
+        if (C::kSplit > 1) bar_sync(1 + stream, 32 * C::kSplit);      // the other warp has read the last record
+        else __syncwarp();
+        float *ow = reinterpret_cast<float *>(my_ring) + part * (kRows * C::kPad);
 #pragma unroll
         for (int gr = 0; gr < G; gr++)
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const int d = gr * 64 + 8 * g + 2 * j;
-                *reinterpret_cast<float2 *>(ow + (2 * t) * C::kPad + d) = make_float2(o[gr][j][0], o[gr][j][2]);
-                *reinterpret_cast<float2 *>(ow + (2 * t + 1) * C::kPad + d) = make_float2(o[gr][j][1], o[gr][j][3]);
+                *reinterpret_cast<float2 *>(ow + (2 * t) * C::kPad + d) =
+                    make_float2(o[gr][j][0] * kEven, o[gr][j][2] * kOdd);
+                *reinterpret_cast<float2 *>(ow + (2 * t + 1) * C::kPad + d) =
+                    make_float2(o[gr][j][1] * kEven, o[gr][j][3] * kOdd);
             }
         __syncthreads();
-        float *slot = p.slots + (long long)(2 * blockIdx.x + (starts ? 1 : 0)) * C::kSlot;
-        for (int i = tid; i < kRows * HD / 8; i += kThreads) {
-            const int r = i / (HD / 8), d = i % (HD / 8) * 8;
+        float *slot = p.slots + (long long)(2 * blockIdx.x + (it.starts ? 1 : 0)) * C::kSlot;
+        if (qr < kRows) {                       // a thread finishes four pairs of a row, a warp 64 in a row at a time
+            const int r = qr;
             float mt = sm_m[0][r];
 #pragma unroll
-            for (int k = 1; k < kWarps; k++) mt = fmaxf(mt, sm_m[k][r]);
+            for (int k = 1; k < kStreams; k++) mt = fmaxf(mt, sm_m[k][r]);
             const float ref = mt == -INFINITY ? 0.0f : mt;
-            float lt = 0.0f, x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+            float lt = 0.0f;
+            float2 x[4] = {};
+            const float *src = reinterpret_cast<const float *>(ring) + r * C::kPad + 2 * qc;
 #pragma unroll
-            for (int k = 0; k < kWarps; k++) {
+            for (int k = 0; k < kStreams; k++) {
                 const float f = ex2(sm_m[k][r] - ref);
                 lt = fmaf(f, sm_l[k][r], lt);
-                const float *src = reinterpret_cast<const float *>(ring + k * (ST * REC)) + r * C::kPad + d;
 #pragma unroll
-                for (int j = 0; j < 8; j++) x[j] = fmaf(f, src[j], x[j]);
+                for (int j = 0; j < 4; j++) {
+                    constexpr int Q = HD / 4;
+                    const float2 y = *reinterpret_cast<const float2 *>(
+                        src + k * (ST * REC / 4) + (j * Q / DW) * (kRows * C::kPad) + j * Q % DW);
+                    x[j].x = fmaf(f, y.x, x[j].x);
+                    x[j].y = fmaf(f, y.y, x[j].y);
+                }
             }
-            if (whole) {
-                if (r < valid) {
+            if (it.whole) {
+                if (r < it.valid) {
                     const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
+                    const unsigned ri = it.tile * kRows + r, tok = ri / group;
+                    const long long to = (it.row0 + (long long)tok) * p.out_stride +
+                                         (long long)(it.h * group + (ri - tok * group)) * HD + 2 * qc;
 #pragma unroll
-                    for (int j = 0; j < 8; j++) x[j] *= inv;
-                    const long long ri = (long long)tile * kRows + r;
-                    store8(p.out, p.type,
-                           (s.row0 + ri / group) * p.out_stride + (long long)(h * group + ri % group) * HD + d, x);
+                    for (int j = 0; j < 4; j++) store2(p.out, p.type, to + j * (HD / 4), x[j].x * inv, x[j].y * inv);
                 }
             } else {
-                if (d == 0) {
+                if (qc == 0) {
                     slot[r] = mt;
                     slot[kRows + r] = lt;
                 }
-                Kv4Vec<float>::store(slot + 2 * kRows + r * HD + d, x);
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    *reinterpret_cast<float2 *>(slot + 2 * kRows + r * HD + 2 * qc + j * (HD / 4)) = x[j];
             }
         }
+        fence_async();                          // the ring is the copies' again
         __syncthreads();
     }
 }
 
-// Joins the partial results of an item that CTAs c - 1, c, ... share. Block
-// (c, r) does row r of the item that is cut at CTA c's start, if c is the first
-// CTA to start inside it.
+// Joins the partial results of the items that are cut between CTAs. Block c - 1
+// looks at the cut at CTA c's start. The K - 1 blocks whose cuts lie in an item of
+// K parts share its 8 x HD outputs evenly, so a block reads about one part's worth
+// whether an item has two parts or 148.
 template <int HD>
-__global__ void __launch_bounds__(128) k_kv4_attn_join(const __grid_constant__ AttnP p) {
+__global__ void __launch_bounds__(kJoinThreads) k_kv4_attn_join(const __grid_constant__ AttnP p) {
     using C = Cfg<HD>;
-    __shared__ Scan<128> scan;
-    griddep_wait();
-    const int c = blockIdx.x + 1, r = blockIdx.y, tid = threadIdx.x;
-    const int per = (p.c.n + 127) / 128;
+    constexpr int NV = kRows * HD / 8;                 // pieces of 8 outputs
+    __shared__ Scan<kJoinThreads> scan;
+    __shared__ float sm_f[C::kCtas * kRows], sm_l[kRows], sm_x[kJoinThreads * 8];
+    const int c = blockIdx.x + 1, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int per = (p.c.n + kJoinThreads - 1) / kJoinThreads;
     long long before, mine;
     const long long total = scan_total(p, scan, per, before, mine);
     const long long share = share_of(total, C::kCtas);
     const long long w = c * share;
     if (w >= total) return;
-    const Where at = find_work(p, scan, per, total, before, mine, w);
-    const Seq s = seq_of(p, at.seq);
-    const int item = (int)(at.off / s.recs), inside = (int)(at.off % s.recs);
-    if (inside == 0 || inside > share) return;        // not cut here, or cut before too
+    find_work(p, scan, per, before, mine, w);
+    const Seq s = seq_of(p, scan.seq);
+    int item, inside;
+    divide(scan.off, s.recs + kItemCost, item, inside);
+    inside -= kItemCost;                               // records of the item before the cut
+    if (inside <= 0) return;                           // not a cut
     const int tile = item / p.c.kv_heads, h = item % p.c.kv_heads;
-    const long long ri = (long long)tile * kRows + r;
-    if (ri >= (long long)s.q * p.group) return;
-    const long long end = w - inside + s.recs;        // first unit behind the item
-    const int last = (int)((end - 1) / share);        // CTAs c - 1 .. last hold parts
-    const float *first = p.slots + (long long)(2 * (c - 1) + 1) * C::kSlot;
-    auto part = [&](int k) { return k == c - 1 ? first : p.slots + (long long)(2 * k) * C::kSlot; };
-    float mt = -INFINITY;
-    for (int k = c - 1; k <= last; k++) mt = fmaxf(mt, part(k)[r]);
-    const float ref = mt == -INFINITY ? 0.0f : mt;
-    const long long at_out = (s.row0 + ri / p.group) * p.out_stride + (long long)(h * p.group + ri % p.group) * HD;
-    for (int d = tid * 8; d < HD; d += 128 * 8) {
-        float lt = 0.0f, x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-        for (int k = c - 1; k <= last; k++) {
-            const float *q = part(k);
-            const float f = ex2(q[r] - ref);
-            float y[8];
-            Kv4Vec<float>::load(q + 2 * kRows + r * HD + d, y);
-            lt = fmaf(f, q[kRows + r], lt);
-#pragma unroll
-            for (int j = 0; j < 8; j++) x[j] = fmaf(f, y[j], x[j]);
+    // CTAs c0, c0 + 1, ... hold the parts: the item's records are the units from w - inside on
+    const int ahead = (int)min(share, 1ll << 30);
+    const int c0 = c - (inside + ahead - 1) / ahead;
+    const int parts = c - c0 + (s.recs - inside + ahead - 1) / ahead;
+    const int nv = (NV + parts - 2) / (parts - 1);     // pieces of this block: [v0, v1)
+    const int v0 = (c - c0 - 1) * nv, v1 = min(NV, v0 + nv);
+    const unsigned group = p.group;
+    auto part = [&](int k) { return p.slots + (long long)(2 * (c0 + k) + (k == 0)) * C::kSlot; };
+    griddep_wait();                                    // the schedule needs no partial result
+    if (warp < kRows) {
+        const int r = warp;
+        float mt = -INFINITY;
+        for (int k = lane; k < parts; k += 32) mt = fmaxf(mt, part(k)[r]);
+        mt = warp_max(mt);
+        const float ref = mt == -INFINITY ? 0.0f : mt;
+        float lt = 0.0f;
+        for (int k = lane; k < parts; k += 32) {
+            const float f = ex2(part(k)[r] - ref);
+            sm_f[k * kRows + r] = f;
+            lt = fmaf(f, part(k)[kRows + r], lt);
         }
-        const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
+        lt = warp_sum(lt);
+        if (lane == 0) sm_l[r] = lt == 0.0f ? 0.0f : 1.0f / lt;
+    }
+    __syncthreads();
+    const int width = min(nv, kJoinThreads), groups = kJoinThreads / width;     // threads of a group: one piece each
+    const int grp = tid / width;
+    for (int vb = v0; vb < v1; vb += width) {
+        const int v = vb + tid % width, r = v / (HD / 8), d = v % (HD / 8) * 8;
+        float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+        if (grp < groups && v < v1) {
+#pragma unroll 4
+            for (int k = grp; k < parts; k += groups) {
+                float y[8];
+                Kv4Vec<float>::load(part(k) + 2 * kRows + r * HD + d, y);
+                const float f = sm_f[k * kRows + r];
 #pragma unroll
-        for (int j = 0; j < 8; j++) x[j] *= inv;
-        store8(p.out, p.type, at_out + d, x);
+                for (int j = 0; j < 8; j++) x[j] = fmaf(f, y[j], x[j]);
+            }
+        }
+        if (groups > 1) {
+            Kv4Vec<float>::store(sm_x + tid * 8, x);
+            __syncthreads();
+            if (grp == 0)
+                for (int k = 1; k < min(groups, parts); k++) {
+                    float y[8];
+                    Kv4Vec<float>::load(sm_x + (k * width + tid) * 8, y);
+#pragma unroll
+                    for (int j = 0; j < 8; j++) x[j] += y[j];
+                }
+        }
+        const unsigned ri = tile * kRows + r;
+        if (grp == 0 && v < v1 && ri < (unsigned)s.q * p.group) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[j] *= sm_l[r];
+            store8(p.out, p.type,
+                       (s.row0 + (long long)(ri / group)) * p.out_stride + (long long)(h * group + ri % group) * HD + d, x);
+        }
     }
 }
 
 template <int HD, bool HILO>
 cudaError_t launch_stream(const AttnP &p, cudaStream_t st) {
     using C = Cfg<HD>;
-    const int smem = C::kRing + (HILO ? 2 : 1) * C::kQ + C::G * 32;
+    const int smem = C::kRing + (HILO ? 2 : 1) * C::kQ + HD / kKv4Group * 32;
     cudaError_t e = g4_smem_optin((const void *)k_kv4_attn<HD, HILO>, smem);
     if (e != cudaSuccess) return e;
-    e = g4_launch(k_kv4_attn<HD, HILO>, dim3(C::kCtas), dim3(kThreads), (size_t)smem, st, false, p);
+    e = g4_launch(k_kv4_attn<HD, HILO>, dim3(C::kCtas), dim3(C::kThreads), (size_t)smem, st, false, p);
     if (e != cudaSuccess) return e;
-    return g4_launch(k_kv4_attn_join<HD>, dim3(C::kCtas - 1, kRows), dim3(128), 0, st, true, p);
+    return g4_launch(k_kv4_attn_join<HD>, dim3(C::kCtas - 1), dim3(kJoinThreads), 0, st, true, p);
 }
 
 template <int HD>
