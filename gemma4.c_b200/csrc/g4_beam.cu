@@ -104,6 +104,7 @@ __global__ void __launch_bounds__(kThreads) k_beam_rows(BeamArgs a) {
     __shared__ uint64_t wkey[kThreads / 32];
     __shared__ int count;
     __shared__ uint32_t s_tau;
+    griddep_wait();
     const int row = blockIdx.x / a.slices, slice = blockIdx.x % a.slices;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const T *p = reinterpret_cast<const T *>(a.logits) + row * a.stride;
@@ -314,8 +315,8 @@ template <typename T>
 cudaError_t launch_rows(const BeamArgs &a, long long rows, cudaStream_t st) {
     const dim3 grid((unsigned)(rows * a.slices)), block(kThreads);
     const bool vec = ((uintptr_t)a.logits & 15) == 0 && a.stride * sizeof(T) % 16 == 0;
-    return vec ? g4_launch(k_beam_rows<T, 16, true>, grid, block, 0, st, false, a)
-               : g4_launch(k_beam_rows<T, 16, false>, grid, block, 0, st, false, a);
+    return vec ? g4_launch(k_beam_rows<T, 16, true>, grid, block, 0, st, true, a)
+               : g4_launch(k_beam_rows<T, 16, false>, grid, block, 0, st, true, a);
 }
 
 }  // namespace

@@ -92,6 +92,7 @@ G4_DEV uint32_t pack8(const float *x, float s, float inv, bool nan) {
 template <typename T>
 __global__ void __launch_bounds__(kThreads) k_kv4_write(Kv4View c, const T *k, long long k_stride, const T *v,
                                                         long long v_stride, int parts) {
+    griddep_wait();
     const int slot = blockIdx.x / parts;
     const int unit = (blockIdx.x % parts) * (kThreads / 32) + (threadIdx.x >> 5);
     const int G = c.hd / kKv4Group;
@@ -173,6 +174,7 @@ G4_DEV void unpack8(uint32_t w, float s, float (&x)[8]) {
 template <typename T>
 __global__ void __launch_bounds__(kThreads) k_kv4_read(Kv4View c, T *k, long long k_stride, T *v, long long v_stride,
                                                        int parts) {
+    griddep_wait();
     const int slot = blockIdx.x / parts;
     const int unit = (blockIdx.x % parts) * (kThreads / 32) + (threadIdx.x >> 5);
     const int G = c.hd / kKv4Group;
@@ -232,6 +234,7 @@ struct ReorderArgs {
 // l, block (i, layers) writes its table row and spare page. Source pages are
 // read only: a destination is a spare page, and no beam's table names one.
 __global__ void __launch_bounds__(256) k_kv4_reorder(const __grid_constant__ ReorderArgs a) {
+    griddep_wait();
     const int i = blockIdx.x, layer = blockIdx.y;
     const int grp = i / a.beams;
     int p = a.parents[i];
@@ -273,9 +276,9 @@ cudaError_t launch_move(bool write, const Kv4View &c, const void *k, long long k
     // rows <= 2^22, n <= 2^16 and parts <= 1024: below 2^31
     const unsigned blocks = (unsigned)((c.rows / kKv4Rec + 2 * c.n) * parts);
     if (write)
-        return g4_launch(k_kv4_write<T>, dim3(blocks), dim3(kThreads), 0, st, false, c, (const T *)k, ks,
+        return g4_launch(k_kv4_write<T>, dim3(blocks), dim3(kThreads), 0, st, true, c, (const T *)k, ks,
                          (const T *)v, vs, parts);
-    return g4_launch(k_kv4_read<T>, dim3(blocks), dim3(kThreads), 0, st, false, c, (T *)k, ks, (T *)v, vs,
+    return g4_launch(k_kv4_read<T>, dim3(blocks), dim3(kThreads), 0, st, true, c, (T *)k, ks, (T *)v, vs,
                      parts);
 }
 
@@ -462,7 +465,7 @@ int g4_kv4_reorder(const g4_kv4_cache *caches, int layers, int groups, int beams
     a.table_out = table_out;
     a.spare_out = spare_out;
     const cudaError_t e = g4_launch(k_kv4_reorder, dim3((unsigned)rows, layers + 1), dim3(256), 0,
-                                    (cudaStream_t)stream, false, a);
+                                    (cudaStream_t)stream, true, a);
     return e == cudaSuccess ? G4_OK : G4_ERR_CUDA;
 }
 

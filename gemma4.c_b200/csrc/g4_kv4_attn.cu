@@ -38,34 +38,27 @@
 namespace {
 
 constexpr int kRows = 8;          // query rows of a tile (tokens x heads of one kv head)
-constexpr int kStreams = 8;       // records in work at a time in one CTA
+constexpr int kStreams = 8;       // warps of a CTA, each with a record of its own
+constexpr int kThreads = kStreams * 32;
 constexpr int kSms = 148;
-constexpr int kJoinThreads = 256;
+constexpr int kJoinThreads = 512;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 8.0f;                      // log2 of how far p may pass 1
 constexpr float kUp = 80.0f;                        // p is 2^80 times too large
 constexpr float kEven = 0x1p53f, kOdd = 0x1p49f;    // outputs: 2^133 / 2^80, 16 times less for odd dimensions
 
-// A record is worked on by kSplit warps, each for kDw dimensions of keys and
-// values: 512 dimensions take two, because the output of 8 rows x 512 in one
-// warp's registers leaves room for only 8 warps on an SM, too few to hide the
-// chain of a record (131072 keys: 32 us with one warp, see the figures below).
 template <int HD>
 struct Cfg {
-    static constexpr int kSplit = HD == 512 ? 2 : 1;
-    static constexpr int kDw = HD / kSplit;
-    static constexpr int G = kDw / kKv4Group;                   // groups of a warp
-    static constexpr int kWarps = kStreams * kSplit;
-    static constexpr int kThreads = kWarps * 32;
+    static constexpr int G = HD / kKv4Group;
     static constexpr int kRec = 17 * HD;
     static constexpr int kStages = HD >= 256 ? 3 : HD == 128 ? 4 : 6;
     static constexpr int kOcc = HD == 512 ? 1 : 2;
     static constexpr int kCtas = kSms * kOcc;
     static constexpr int kRing = kStreams * kStages * kRec;
-    static constexpr int kQ = HD / kKv4Group * 1024;            // operands of the query tile (one half)
-    static constexpr int kPad = kDw + 2;                        // row of a warp's output when the warps meet
-    static constexpr int kSlot = 2 * kRows + kRows * HD;        // floats of one partial result
-    static_assert(kStages * kRec >= kSplit * kRows * kPad * 4, "a stream's ring holds its output tile");
+    static constexpr int kQ = G * 1024;                         // operands of the query tile (one half)
+    static constexpr int kPad = HD + 2;                        // row of a warp's output when the warps meet
+    static constexpr int kSlot = kRows * HD;                    // floats of one partial output
+    static_assert(kStages * kRec >= kRows * kPad * 4, "a stream's ring holds its output tile");
 };
 
 struct AttnP {
@@ -77,7 +70,8 @@ struct AttnP {
     long long q_stride, out_stride;
     float scale;
     int window;
-    float *slots;                 // partial results, two per CTA
+    float *slots;                 // partial outputs [2 per CTA][8][HD]
+    float *stats;                 // their maxima and sums [2 per CTA][2][8]
 };
 
 G4_DEV void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
@@ -165,7 +159,14 @@ G4_DEV void store2(void *p, int type, long long i, float x, float y) {
 // N bf16 scales, and one of a pair as fp32
 template <int N>
 G4_DEV void load_scales(const void *p, uint32_t (&w)[(N + 1) / 2]) {
-    if constexpr (N == 4) {
+    static_assert(N == 8 || N == 4 || N == 2 || N == 1, "the groups of a head");
+    if constexpr (N == 8) {
+        const uint4 x = *reinterpret_cast<const uint4 *>(p);
+        w[0] = x.x;
+        w[1] = x.y;
+        w[2] = x.z;
+        w[3] = x.w;
+    } else if constexpr (N == 4) {
         const uint2 x = *reinterpret_cast<const uint2 *>(p);
         w[0] = x.x;
         w[1] = x.y;
@@ -343,26 +344,27 @@ G4_DEV void next_item(const AttnP &p, Walk &w, Item &out) {
 }
 
 template <int HD, bool HILO>
-__global__ void __launch_bounds__(Cfg<HD>::kThreads, Cfg<HD>::kOcc) k_kv4_attn(const __grid_constant__ AttnP p) {
+__global__ void __launch_bounds__(kThreads, Cfg<HD>::kOcc) k_kv4_attn(const __grid_constant__ AttnP p) {
     using C = Cfg<HD>;
-    constexpr int G = C::G, REC = C::kRec, ST = C::kStages, DW = C::kDw, HG = HD / kKv4Group;
+    constexpr int G = C::G, REC = C::kRec, ST = C::kStages;
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t *ring = smem;
     uint4 *qhi = reinterpret_cast<uint4 *>(smem + C::kRing);            // [HD / 64][2][32] (lane's operands of two steps)
     uint4 *qlo = qhi + C::kQ / 16;
     float *qoff = reinterpret_cast<float *>(smem + C::kRing + (HILO ? 2 : 1) * C::kQ);   // [HD / 64][8]: -8 sum q
-    __shared__ Scan<C::kThreads> scan;
+    __shared__ Scan<kThreads> scan;
     __shared__ Walk walk;
     __shared__ Item items[2];
-    __shared__ float row_scale[kRows], row_max[C::kWarps], sm_m[kStreams][kRows], sm_l[kStreams][kRows];
+    __shared__ float row_scale[kRows], row_max[2][kStreams], sm_m[kStreams][kRows], sm_l[kStreams][kRows];
     __shared__ uint64_t full[kStreams][ST];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int stream = warp / C::kSplit, part = warp % C::kSplit;       // this warp: groups [part * G, + G)
+    const int stream = warp;
     const unsigned group = p.group;
 
     if (tid < kStreams * ST) mbar_init(&full[0][0] + tid, 1);
     mbar_fence_init();
-    const int per = (p.c.n + C::kThreads - 1) / C::kThreads;
+    griddep_wait();
+    const int per = (p.c.n + kThreads - 1) / kThreads;
     long long before, mine;
     const long long total = scan_total(p, scan, per, before, mine);
     const long long share = share_of(total, C::kCtas);
@@ -370,7 +372,7 @@ __global__ void __launch_bounds__(Cfg<HD>::kThreads, Cfg<HD>::kOcc) k_kv4_attn(c
     griddep_launch();
     if (w0 >= total) return;
     find_work(p, scan, per, before, mine, w0);
-    if (warp == C::kWarps - 1) {
+    if (warp == kStreams - 1) {
         if (lane == 0) {
             walk.left = min(total - w0, share);
             walk.b = scan.seq;
@@ -388,9 +390,11 @@ __global__ void __launch_bounds__(Cfg<HD>::kThreads, Cfg<HD>::kOcc) k_kv4_attn(c
         const int rec = it.ra + stream + (k0 + lane) * kStreams;
         return rec < it.rb ? (unsigned long long)kv4_record(p.c, it.b, (long long)rec * 16, it.h) : 0;
     };
-    // 8 dimensions of a query row per thread
-    const int qr = tid / (HD / 8), qc = tid % (HD / 8);
-    auto load_q = [&](const Item &it, float (&x)[8]) {
+    // 8 dimensions of a query row per thread and pass
+    constexpr int QN = kRows * HD / 8 > kThreads ? kRows * HD / 8 / kThreads : 1;
+    const int qc = tid % (HD / 8);
+    auto load_q = [&](const Item &it, float (&x)[8], int pass) {
+        const int qr = tid / (HD / 8) + pass * (kRows / QN);
 #pragma unroll
         for (int i = 0; i < 8; i++) x[i] = 0.0f;
         if (qr < it.valid) {
@@ -400,10 +404,11 @@ __global__ void __launch_bounds__(Cfg<HD>::kThreads, Cfg<HD>::kOcc) k_kv4_attn(c
     };
 
     unsigned long long addr = 0;
-    float qx[8];
+    float qx[QN][8];
     if (!items[0].none) {
         addr = lookup(items[0], 0);
-        load_q(items[0], qx);
+#pragma unroll
+        for (int i = 0; i < QN; i++) load_q(items[0], qx[i], i);
     }
     for (int cur = 0; !items[cur].none; cur ^= 1) {
         const Item &it = items[cur];
@@ -416,37 +421,41 @@ __global__ void __launch_bounds__(Cfg<HD>::kThreads, Cfg<HD>::kOcc) k_kv4_attn(c
             const uint8_t *src = (const uint8_t *)__shfl_sync(0xffffffffu, addr, k & 31);
             const int st = k % ST;
             there = src ? there | 1u << st : there & ~(1u << st);
-            if (src && part == 0 && lane == 0) {
+            if (src && lane == 0) {
                 mbar_arrive_expect_tx(&full[stream][st], REC);
                 bulk_load(my_ring + st * REC, src, REC, &full[stream][st]);
             }
         };
-        for (int k = 0; k < ST - 1; k++) issue(k);
-        if (warp == C::kWarps - 1) next_item(p, walk, items[cur ^ 1]);
+        for (int k = 0; k < ST; k++) issue(k);
+        if (warp == kStreams - 1) next_item(p, walk, items[cur ^ 1]);
 
         // query operands
-        {
+#pragma unroll
+        for (int pass = 0; pass < QN; pass++) {
+            const float (&x)[8] = qx[pass];
+            const int qr = tid / (HD / 8) + pass * (kRows / QN);
             float mx = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 8; i++) mx = fmaxf(mx, fabsf(qx[i]));
+            for (int i = 0; i < 8; i++) mx = fmaxf(mx, fabsf(x[i]));
 #pragma unroll
             for (int o = 1; o < min(32, HD / 8); o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
             if constexpr (HD / 8 > 32) {
-                if (lane == 0) row_max[warp] = mx;
+                if (lane == 0) row_max[pass][warp] = mx;
                 __syncthreads();
-                mx = fmaxf(mx, row_max[warp ^ 1]);
+                mx = fmaxf(mx, row_max[pass][warp ^ 1]);
             }
             // exact power of two that brings the row's largest |q| to 2^13..2^14
             const int e = min(max((int)(__float_as_uint(mx) >> 23) - 127, -100), 115);
-            const float up = __uint_as_float((uint32_t)(127 + 13 - e) << 23);
+            // (the sign of the softmax scale goes with it, so that row_scale is positive)
+            const float up = copysignf(__uint_as_float((uint32_t)(127 + 13 - e) << 23), p.scale);
             // 8 dimensions: group qc / 8, t = qc / 2 % 4, half qc % 2; steps 2 half + i take
             // dimensions 2i, 2i+4 and, a nibble up, 2i+1, 2i+5
             float rep = 0.0f;
             uint32_t hi[4], lo[4];
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                const float y[4] = {qx[2 * i] * up, qx[2 * i + 4] * up, qx[2 * i + 1] * up * 0.0625f,
-                                    qx[2 * i + 5] * up * 0.0625f};
+                const float y[4] = {x[2 * i] * up, x[2 * i + 4] * up, x[2 * i + 1] * up * 0.0625f,
+                                    x[2 * i + 5] * up * 0.0625f};
                 hi[2 * i] = pack_h(y[0], y[1]);
                 hi[2 * i + 1] = pack_h(y[2], y[3]);
                 float2 f0 = unpack_h(hi[2 * i]), f1 = unpack_h(hi[2 * i + 1]);
@@ -463,7 +472,7 @@ __global__ void __launch_bounds__(Cfg<HD>::kThreads, Cfg<HD>::kOcc) k_kv4_attn(c
             for (int o = 1; o < 8; o <<= 1) rep += __shfl_xor_sync(0xffffffffu, rep, o);
             if (qr < kRows) {
                 if (qc == 0)
-                    row_scale[qr] = p.scale * kLog2e * __uint_as_float((uint32_t)(127 + 24 - 13 + e) << 23);
+                    row_scale[qr] = fabsf(p.scale) * kLog2e * __uint_as_float((uint32_t)(127 + 24 - 13 + e) << 23);
                 const int to = ((qc >> 3) * 2 + (qc & 1)) * 32 + qr * 4 + (qc >> 1 & 3);
                 qhi[to] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
                 if (HILO) qlo[to] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
@@ -485,170 +494,141 @@ __global__ void __launch_bounds__(Cfg<HD>::kThreads, Cfg<HD>::kOcc) k_kv4_attn(c
 #pragma unroll
                 for (int k = 0; k < 4; k++) o[i][j][k] = 0.0f;
         float m = -INFINITY, l = 0.0f;
-        const float rs0 = row_scale[2 * t], rs1 = row_scale[2 * t + 1];
+        const float rs = row_scale[g];
 
         bool lost = false;                                    // a copy that never came
+        uint32_t ph0 = 0, ph1 = 0, pl0 = 0, pl1 = 0;          // p of a record as high and low bf16
+        uint32_t see01 = 0, see23 = 0;                        // which of its keys row g sees, as masks of the scales
+
+        // scores of one group: lane holds keys g, g + 8 x rows 2t, 2t + 1
+        auto score = [&](const uint8_t *rec, int gr, const uint32_t (&k0s)[(G + 1) / 2],
+                         const uint32_t (&k1s)[(G + 1) / 2], float (&sc)[4]) {
+            const uint4 kc = *reinterpret_cast<const uint4 *>(rec + gr * 512 + lane * 16);
+            const float2 q0 = *reinterpret_cast<const float2 *>(qoff + gr * 8 + 2 * t);
+            float d[4] = {q0.x, q0.y, q0.x, q0.y};
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+                uint32_t x = half ? kc.y : kc.x, z = half ? kc.w : kc.z;
+                const int qi = (gr * 2 + half) * 32 + lane;
+                const uint4 bh = qhi[qi];
+                uint4 bl;
+                if (HILO) bl = qlo[qi];
+                const uint32_t a0 = x & 0x000f000fu, a1 = z & 0x000f000fu, a2 = x & 0x00f000f0u, a3 = z & 0x00f000f0u;
+                mma_h(d, a0, a1, a2, a3, bh.x, bh.y);
+                if (HILO) mma_h(d, a0, a1, a2, a3, bl.x, bl.y);
+                x >>= 8;
+                z >>= 8;
+                const uint32_t a4 = x & 0x000f000fu, a5 = z & 0x000f000fu, a6 = x & 0x00f000f0u, a7 = z & 0x00f000f0u;
+                mma_h(d, a4, a5, a6, a7, bh.z, bh.w);
+                if (HILO) mma_h(d, a4, a5, a6, a7, bl.z, bl.w);
+            }
+            const float k0 = half_of(k0s[gr / 2], gr & 1), k1 = half_of(k1s[gr / 2], gr & 1);
+            sc[0] = fmaf(d[0], k0, sc[0]);
+            sc[1] = fmaf(d[1], k0, sc[1]);
+            sc[2] = fmaf(d[2], k1, sc[2]);
+            sc[3] = fmaf(d[3], k1, sc[3]);
+        };
+        // output of one group: lane holds dimensions 8g + 2j, + 1 x rows 2t, 2t + 1
+        auto value = [&](const uint8_t *rec, int gr) {
+            const uint4 vc = *reinterpret_cast<const uint4 *>(rec + 8 * HD + gr * 512 + lane * 16);
+            uint2 vs = reinterpret_cast<const uint2 *>(rec + 16 * HD + 32 * G)[gr * 4 + t];
+            vs.x &= see01;                                    // the scale of a token that is not seen may be anything
+            vs.y &= see23;
+            // p vs = h + l: h the rounded product of p's high half, l what it lost and the low half's product
+            const uint32_t h0 = mul_b(ph0, vs.x), h1 = mul_b(ph1, vs.y);
+            const uint32_t l0 = fma_b(pl0, vs.x, fma_b(ph0, vs.x, h0 ^ 0x80008000u));
+            const uint32_t l1 = fma_b(pl1, vs.y, fma_b(ph1, vs.y, h1 ^ 0x80008000u));
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const uint32_t ab = __byte_perm(vc.x, vc.y, j < 2 ? 0x5410 : 0x7632) >> (8 * (j & 1));
+                const uint32_t cd = __byte_perm(vc.z, vc.w, j < 2 ? 0x5410 : 0x7632) >> (8 * (j & 1));
+                const uint32_t a0 = code_lo(ab), a1 = code_hi(ab), a2 = code_lo(cd), a3 = code_hi(cd);
+                mma_b(o[gr][j], a0, a1, a2, a3, h0, h1);
+                mma_b(o[gr][j], a0, a1, a2, a3, l0, l1);
+            }
+        };
+
+        int st = 0;
         for (int k = 0; k < nmine; k++) {
-            const int st = k % ST;
-            if (C::kSplit == 1) {
-                __syncwarp();
-                issue(k + ST - 1);
-            }
-            if (!(there >> st & 1)) {                         // no page: no keys (for all warps of the record)
-                if (C::kSplit > 1) {
-                    bar_sync(1 + stream, 32 * C::kSplit);
-                    issue(k + ST - 1);
-                }
-                continue;
-            }
-            if (!mbar_wait(&full[stream][st], phase >> st & 1, nullptr, 0)) lost = true;
-            phase ^= 1u << st;
-            uint8_t *rec = my_ring + st * REC;
-            const int key0 = (ra + stream + k * kStreams) * 16;
-
-            // ---- scores: lane holds keys g, g + 8 x rows 2t, 2t + 1 ----
-            float sc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            uint32_t k0s[(G + 1) / 2], k1s[(G + 1) / 2];      // scales of keys g and g + 8
-            load_scales<G>(rec + 16 * HD + g * (2 * HG) + part * (2 * G), k0s);
-            load_scales<G>(rec + 16 * HD + (g + 8) * (2 * HG) + part * (2 * G), k1s);
+            const uint8_t *rec = my_ring + st * REC;
+            const bool here = there >> st & 1;                // a missing page has no keys
+            if (here) {
+                if (!mbar_wait(&full[stream][st], phase >> st & 1, nullptr, 0)) lost = true;
+                phase ^= 1u << st;
+                float sc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                uint32_t k0s[(G + 1) / 2], k1s[(G + 1) / 2];  // scales of keys g and g + 8
+                load_scales<G>(rec + 16 * HD + g * (2 * G), k0s);
+                load_scales<G>(rec + 16 * HD + (g + 8) * (2 * G), k1s);
 #pragma unroll
-            for (int gr = 0; gr < G; gr++) {
-                const uint4 kc = *reinterpret_cast<const uint4 *>(rec + (part * G + gr) * 512 + lane * 16);
-                const float2 q0 = *reinterpret_cast<const float2 *>(qoff + (part * G + gr) * 8 + 2 * t);
-                float d[4] = {q0.x, q0.y, q0.x, q0.y};
+                for (int gr = 0; gr < G; gr++) score(rec, gr, k0s, k1s, sc);
+                // row g, keys 2t, 2t + 1, 2t + 8, 2t + 9
+                transpose2(sc[0], sc[1]);
+                transpose2(sc[2], sc[3]);
+                const int key0 = (ra + stream + k * kStreams) * 16;
+                see01 = see23 = 0xffffffffu;
+                if (key0 < all0 || key0 + 15 > all1) {
+                    see01 = see23 = 0;
 #pragma unroll
-                for (int half = 0; half < 2; half++) {
-                    uint32_t x = half ? kc.y : kc.x, z = half ? kc.w : kc.z;
-                    const int qi = ((part * G + gr) * 2 + half) * 32 + lane;
-                    const uint4 bh = qhi[qi];
-                    uint4 bl;
-                    if (HILO) bl = qlo[qi];
-                    const uint32_t a0 = x & 0x000f000fu, a1 = z & 0x000f000fu, a2 = x & 0x00f000f0u,
-                                   a3 = z & 0x00f000f0u;
-                    mma_h(d, a0, a1, a2, a3, bh.x, bh.y);
-                    if (HILO) mma_h(d, a0, a1, a2, a3, bl.x, bl.y);
-                    x >>= 8;
-                    z >>= 8;
-                    const uint32_t a4 = x & 0x000f000fu, a5 = z & 0x000f000fu, a6 = x & 0x00f000f0u,
-                                   a7 = z & 0x00f000f0u;
-                    mma_h(d, a4, a5, a6, a7, bh.z, bh.w);
-                    if (HILO) mma_h(d, a4, a5, a6, a7, bl.z, bl.w);
-                }
-                const float k0 = half_of(k0s[gr / 2], gr & 1), k1 = half_of(k1s[gr / 2], gr & 1);
-                sc[0] = fmaf(d[0], k0, sc[0]);
-                sc[1] = fmaf(d[1], k0, sc[1]);
-                sc[2] = fmaf(d[2], k1, sc[2]);
-                sc[3] = fmaf(d[3], k1, sc[3]);
-            }
-            if constexpr (C::kSplit > 1) {
-                // The other warp's groups: both add in the same order. A warp leaves its
-                // scores where its K codes were; the next copy into that stage is issued
-                // behind the barrier of the next record, when they have been read.
-                __syncwarp();
-                float4 *x4 = reinterpret_cast<float4 *>(rec) + lane;
-                x4[part * (8 * DW / 16)] = make_float4(sc[0], sc[1], sc[2], sc[3]);
-                fence_async();
-                bar_sync(1 + stream, 32 * C::kSplit);
-                issue(k + ST - 1);
-                const float4 x = x4[0], y = x4[8 * DW / 16];
-                sc[0] = x.x + y.x;
-                sc[1] = x.y + y.y;
-                sc[2] = x.z + y.z;
-                sc[3] = x.w + y.w;
-            }
-            sc[0] *= rs0;
-            sc[1] *= rs1;
-            sc[2] *= rs0;
-            sc[3] *= rs1;
-            // ---- row g, keys 2t, 2t + 1, 2t + 8, 2t + 9 ----
-            transpose2(sc[0], sc[1]);
-            transpose2(sc[2], sc[3]);
-            const bool edge = key0 < all0 || key0 + 15 > all1;
-            uint32_t see01 = 0, see23 = 0;
-            if (edge) {
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int key = key0 + 2 * t + (i & 1) + 8 * (i >> 1);
-                    const bool see = key >= my_lo && key <= my_hi;
-                    if (!see) sc[i] = -INFINITY;
-                    else if (i < 2) see01 |= 0xffffu << (16 * (i & 1));
-                    else see23 |= 0xffffu << (16 * (i & 1));
-                }
-            }
-            float mx = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            // The reference m follows the maximum when that is kSlack above it: p stays
-            // below 2^kSlack, and the outputs are rescaled a few times per sequence.
-            if (__any_sync(0xffffffffu, mx > m + kSlack)) {
-                const float mn = mx > m + kSlack ? mx : m;
-                const float al = mn == -INFINITY ? 1.0f : ex2(m - mn);
-                m = mn;
-                l *= al;
-                const float al0 = __shfl_sync(0xffffffffu, al, 8 * t), al1 = __shfl_sync(0xffffffffu, al, 8 * t + 4);
-#pragma unroll
-                for (int i = 0; i < G; i++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        o[i][j][0] *= al0;
-                        o[i][j][1] *= al1;
-                        o[i][j][2] *= al0;
-                        o[i][j][3] *= al1;
-                    }
-            }
-            const float mref = (m == -INFINITY ? 0.0f : m) - kUp;
-            float pr[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) pr[i] = ex2(sc[i] - mref);
-            l += (pr[0] + pr[1]) + (pr[2] + pr[3]);
-            // p as high and low bf16
-            const uint32_t ph0 = pack_b(pr[0], pr[1]), ph1 = pack_b(pr[2], pr[3]);
-            const uint32_t pl0 = pack_b(pr[0] - half_of(ph0, 0), pr[1] - half_of(ph0, 1));
-            const uint32_t pl1 = pack_b(pr[2] - half_of(ph1, 0), pr[3] - half_of(ph1, 1));
-
-            // ---- output: lane holds dimensions 8g + 2j, + 1 of each group x rows 2t, 2t + 1 ----
-            const uint2 *vsp = reinterpret_cast<const uint2 *>(rec + 16 * HD + 32 * HG + part * (32 * G)) + t;
-#pragma unroll
-            for (int gr = 0; gr < G; gr++) {
-                const uint4 vc = *reinterpret_cast<const uint4 *>(rec + 8 * HD + (part * G + gr) * 512 + lane * 16);
-                uint2 vs = vsp[gr * 4];
-                if (edge) {                               // the scale of a token that is not seen may be anything
-                    vs.x &= see01;
-                    vs.y &= see23;
-                }
-                // p vs = h + l: h the rounded product of p's high half, l what it lost and the low half's product
-                const uint32_t h0 = mul_b(ph0, vs.x), h1 = mul_b(ph1, vs.y);
-                const uint32_t l0 = fma_b(pl0, vs.x, fma_b(ph0, vs.x, h0 ^ 0x80008000u));
-                const uint32_t l1 = fma_b(pl1, vs.y, fma_b(ph1, vs.y, h1 ^ 0x80008000u));
-#pragma unroll
-                for (int half = 0; half < 2; half++) {
-                    uint32_t ab = __byte_perm(vc.x, vc.y, half ? 0x7632 : 0x5410);
-                    uint32_t cd = __byte_perm(vc.z, vc.w, half ? 0x7632 : 0x5410);
-#pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        const uint32_t a0 = code_lo(ab), a1 = code_hi(ab), a2 = code_lo(cd), a3 = code_hi(cd);
-                        mma_b(o[gr][2 * half + i], a0, a1, a2, a3, h0, h1);
-                        mma_b(o[gr][2 * half + i], a0, a1, a2, a3, l0, l1);
-                        ab >>= 8;
-                        cd >>= 8;
+                    for (int i = 0; i < 4; i++) {
+                        const int key = key0 + 2 * t + (i & 1) + 8 * (i >> 1);
+                        const bool see = key >= my_lo && key <= my_hi;
+                        if (!see) sc[i] = -INFINITY;
+                        else if (i < 2) see01 |= 0xffffu << (16 * (i & 1));
+                        else see23 |= 0xffffu << (16 * (i & 1));
                     }
                 }
+                float mx = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)) * rs;
+                // The reference m follows the maximum when that is kSlack above it: p stays
+                // below 2^kSlack, and the outputs are rescaled a few times per sequence.
+                if (__any_sync(0xffffffffu, mx > m + kSlack)) {
+                    const float mn = mx > m + kSlack ? mx : m;
+                    const float al = mn == -INFINITY ? 1.0f : ex2(m - mn);
+                    m = mn;
+                    l *= al;
+                    const float al0 = __shfl_sync(0xffffffffu, al, 8 * t),
+                                al1 = __shfl_sync(0xffffffffu, al, 8 * t + 4);
+#pragma unroll
+                    for (int i = 0; i < G; i++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            o[i][j][0] *= al0;
+                            o[i][j][1] *= al1;
+                            o[i][j][2] *= al0;
+                            o[i][j][3] *= al1;
+                        }
+                }
+                const float mref = (m == -INFINITY ? 0.0f : m) - kUp;
+                float pr[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) pr[i] = ex2(fmaf(sc[i], rs, -mref));
+                l += (pr[0] + pr[1]) + (pr[2] + pr[3]);
+                ph0 = pack_b(pr[0], pr[1]);
+                ph1 = pack_b(pr[2], pr[3]);
+                pl0 = pack_b(pr[0] - half_of(ph0, 0), pr[1] - half_of(ph0, 1));
+                pl1 = pack_b(pr[2] - half_of(ph1, 0), pr[3] - half_of(ph1, 1));
+#pragma unroll
+                for (int gr = 0; gr < G; gr++) value(rec, gr);
+                __syncwarp();
             }
+            issue(k + ST);                                    // into the stage that is free now
+            st = st + 1 == ST ? 0 : st + 1;
         }
         if (lost) l = NAN;
 
         // ---- the warps meet; the next item's addresses and queries are on their way ----
         if (!items[cur ^ 1].none) {
             addr = lookup(items[cur ^ 1], 0);
-            load_q(items[cur ^ 1], qx);
+#pragma unroll
+            for (int i = 0; i < QN; i++) load_q(items[cur ^ 1], qx[i], i);
         }
         l += __shfl_xor_sync(0xffffffffu, l, 1);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
         l *= 0x1p-80f;
-        if (t == 0 && part == 0) { sm_m[stream][g] = m; sm_l[stream][g] = l; }
-        if (C::kSplit > 1) bar_sync(1 + stream, 32 * C::kSplit);      // the other warp has read the last record
-        else __syncwarp();
-        float *ow = reinterpret_cast<float *>(my_ring) + part * (kRows * C::kPad);
+        if (t == 0) { sm_m[stream][g] = m; sm_l[stream][g] = l; }
+        __syncwarp();
+        float *ow = reinterpret_cast<float *>(my_ring);
 #pragma unroll
         for (int gr = 0; gr < G; gr++)
 #pragma unroll
@@ -660,9 +640,9 @@ __global__ void __launch_bounds__(Cfg<HD>::kThreads, Cfg<HD>::kOcc) k_kv4_attn(c
                     make_float2(o[gr][j][1] * kEven, o[gr][j][3] * kOdd);
             }
         __syncthreads();
-        float *slot = p.slots + (long long)(2 * blockIdx.x + (it.starts ? 1 : 0)) * C::kSlot;
-        if (qr < kRows) {                       // a thread finishes four pairs of a row, a warp 64 in a row at a time
-            const int r = qr;
+        const int slot = 2 * blockIdx.x + (it.starts ? 1 : 0);
+        // a thread finishes four pairs of a row, a warp 64 in a row at a time
+        for (int r = tid / (HD / 8); r < kRows; r += kThreads / (HD / 8)) {
             float mt = sm_m[0][r];
 #pragma unroll
             for (int k = 1; k < kStreams; k++) mt = fmaxf(mt, sm_m[k][r]);
@@ -678,7 +658,7 @@ __global__ void __launch_bounds__(Cfg<HD>::kThreads, Cfg<HD>::kOcc) k_kv4_attn(c
                 for (int j = 0; j < 4; j++) {
                     constexpr int Q = HD / 4;
                     const float2 y = *reinterpret_cast<const float2 *>(
-                        src + k * (ST * REC / 4) + (j * Q / DW) * (kRows * C::kPad) + j * Q % DW);
+                        src + k * (ST * REC / 4) + j * Q);
                     x[j].x = fmaf(f, y.x, x[j].x);
                     x[j].y = fmaf(f, y.y, x[j].y);
                 }
@@ -694,12 +674,13 @@ __global__ void __launch_bounds__(Cfg<HD>::kThreads, Cfg<HD>::kOcc) k_kv4_attn(c
                 }
             } else {
                 if (qc == 0) {
-                    slot[r] = mt;
-                    slot[kRows + r] = lt;
+                    p.stats[slot * (2 * kRows) + r] = mt;
+                    p.stats[slot * (2 * kRows) + kRows + r] = lt;
                 }
 #pragma unroll
                 for (int j = 0; j < 4; j++)
-                    *reinterpret_cast<float2 *>(slot + 2 * kRows + r * HD + 2 * qc + j * (HD / 4)) = x[j];
+                    *reinterpret_cast<float2 *>(p.slots + (long long)slot * C::kSlot + r * HD + 2 * qc +
+                                                j * (HD / 4)) = x[j];
             }
         }
         fence_async();                          // the ring is the copies' again
@@ -716,7 +697,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_kv4_attn_join(const __grid_con
     using C = Cfg<HD>;
     constexpr int NV = kRows * HD / 8;                 // pieces of 8 outputs
     __shared__ Scan<kJoinThreads> scan;
-    __shared__ float sm_f[C::kCtas * kRows], sm_l[kRows], sm_x[kJoinThreads * 8];
+    __shared__ float sm_f[C::kCtas * kRows], sm_l[C::kCtas * kRows], inv[kRows];
     const int c = blockIdx.x + 1, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int per = (p.c.n + kJoinThreads - 1) / kJoinThreads;
     long long before, mine;
@@ -738,56 +719,64 @@ __global__ void __launch_bounds__(kJoinThreads) k_kv4_attn_join(const __grid_con
     const int nv = (NV + parts - 2) / (parts - 1);     // pieces of this block: [v0, v1)
     const int v0 = (c - c0 - 1) * nv, v1 = min(NV, v0 + nv);
     const unsigned group = p.group;
-    auto part = [&](int k) { return p.slots + (long long)(2 * (c0 + k) + (k == 0)) * C::kSlot; };
+    auto slot = [&](int k) { return 2 * (c0 + k) + (k == 0); };
     griddep_wait();                                    // the schedule needs no partial result
-    if (warp < kRows) {
-        const int r = warp;
+    const int ra = v0 / (HD / 8), rn = max(0, (v1 - 1) / (HD / 8) - ra + 1);     // its rows
+    for (int i = tid; i < parts * rn; i += kJoinThreads) {
+        const int k = i / rn, r = ra + i % rn;
+        sm_f[k * kRows + r] = p.stats[slot(k) * (2 * kRows) + r];
+        sm_l[k * kRows + r] = p.stats[slot(k) * (2 * kRows) + kRows + r];
+    }
+    __syncthreads();
+    if (warp < rn) {
+        const int r = ra + warp;
         float mt = -INFINITY;
-        for (int k = lane; k < parts; k += 32) mt = fmaxf(mt, part(k)[r]);
+        for (int k = lane; k < parts; k += 32) mt = fmaxf(mt, sm_f[k * kRows + r]);
         mt = warp_max(mt);
         const float ref = mt == -INFINITY ? 0.0f : mt;
         float lt = 0.0f;
         for (int k = lane; k < parts; k += 32) {
-            const float f = ex2(part(k)[r] - ref);
+            const float f = ex2(sm_f[k * kRows + r] - ref);
             sm_f[k * kRows + r] = f;
-            lt = fmaf(f, part(k)[kRows + r], lt);
+            lt = fmaf(f, sm_l[k * kRows + r], lt);
         }
         lt = warp_sum(lt);
-        if (lane == 0) sm_l[r] = lt == 0.0f ? 0.0f : 1.0f / lt;
+        if (lane == 0) inv[r] = lt == 0.0f ? 0.0f : 1.0f / lt;
     }
     __syncthreads();
-    const int width = min(nv, kJoinThreads), groups = kJoinThreads / width;     // threads of a group: one piece each
-    const int grp = tid / width;
-    for (int vb = v0; vb < v1; vb += width) {
-        const int v = vb + tid % width, r = v / (HD / 8), d = v % (HD / 8) * 8;
+    // `width` lanes share a piece, up to five parts each loaded at once
+    constexpr int kAtOnce = 5;
+    int width = 1;
+    while (width < 32 && width * kAtOnce < parts) width *= 2;
+    const int sub = tid % width;
+    for (int vb = v0; vb < v1; vb += kJoinThreads / width) {
+        const int v = vb + tid / width, r = min(v, v1 - 1) / (HD / 8), d = min(v, v1 - 1) % (HD / 8) * 8;
         float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-        if (grp < groups && v < v1) {
-#pragma unroll 4
-            for (int k = grp; k < parts; k += groups) {
-                float y[8];
-                Kv4Vec<float>::load(part(k) + 2 * kRows + r * HD + d, y);
-                const float f = sm_f[k * kRows + r];
+        for (int kb = 0; kb < parts; kb += kAtOnce * width) {
+            float y[kAtOnce][8];
 #pragma unroll
-                for (int j = 0; j < 8; j++) x[j] = fmaf(f, y[j], x[j]);
+            for (int i = 0; i < kAtOnce; i++) {
+                const int k = kb + i * width + sub;
+                if (k < parts) Kv4Vec<float>::load(p.slots + (long long)slot(k) * C::kSlot + r * HD + d, y[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < kAtOnce; i++) {
+                const int k = kb + i * width + sub;
+                const float f = k < parts ? sm_f[k * kRows + r] : 0.0f;
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    if (k < parts) x[j] = fmaf(f, y[i][j], x[j]);
             }
         }
-        if (groups > 1) {
-            Kv4Vec<float>::store(sm_x + tid * 8, x);
-            __syncthreads();
-            if (grp == 0)
-                for (int k = 1; k < min(groups, parts); k++) {
-                    float y[8];
-                    Kv4Vec<float>::load(sm_x + (k * width + tid) * 8, y);
+        for (int o = 1; o < width; o <<= 1)
 #pragma unroll
-                    for (int j = 0; j < 8; j++) x[j] += y[j];
-                }
-        }
+            for (int j = 0; j < 8; j++) x[j] += __shfl_xor_sync(0xffffffffu, x[j], o);
         const unsigned ri = tile * kRows + r;
-        if (grp == 0 && v < v1 && ri < (unsigned)s.q * p.group) {
+        if (sub == 0 && v < v1 && ri < (unsigned)s.q * group) {
 #pragma unroll
-            for (int j = 0; j < 8; j++) x[j] *= sm_l[r];
+            for (int j = 0; j < 8; j++) x[j] *= inv[r];
             store8(p.out, p.type,
-                       (s.row0 + (long long)(ri / group)) * p.out_stride + (long long)(h * group + ri % group) * HD + d, x);
+                   (s.row0 + (long long)(ri / group)) * p.out_stride + (long long)(h * group + ri % group) * HD + d, x);
         }
     }
 }
@@ -795,22 +784,23 @@ __global__ void __launch_bounds__(kJoinThreads) k_kv4_attn_join(const __grid_con
 template <int HD, bool HILO>
 cudaError_t launch_stream(const AttnP &p, cudaStream_t st) {
     using C = Cfg<HD>;
-    const int smem = C::kRing + (HILO ? 2 : 1) * C::kQ + HD / kKv4Group * 32;
+    const int smem = C::kRing + (HILO ? 2 : 1) * C::kQ + C::G * 32;
     cudaError_t e = g4_smem_optin((const void *)k_kv4_attn<HD, HILO>, smem);
     if (e != cudaSuccess) return e;
-    e = g4_launch(k_kv4_attn<HD, HILO>, dim3(C::kCtas), dim3(C::kThreads), (size_t)smem, st, false, p);
+    e = g4_launch(k_kv4_attn<HD, HILO>, dim3(C::kCtas), dim3(kThreads), (size_t)smem, st, true, p);
     if (e != cudaSuccess) return e;
     return g4_launch(k_kv4_attn_join<HD>, dim3(C::kCtas - 1), dim3(kJoinThreads), 0, st, true, p);
 }
 
 template <int HD>
-cudaError_t launch_hd(const AttnP &p, cudaStream_t st) {
+cudaError_t launch_hd(AttnP &p, cudaStream_t st) {
+    p.stats = p.slots + (size_t)2 * Cfg<HD>::kCtas * Cfg<HD>::kSlot;
     return p.type == G4_TYPE_F32 ? launch_stream<HD, true>(p, st) : launch_stream<HD, false>(p, st);
 }
 
 template <int HD>
 size_t ws_bytes() {
-    return (size_t)2 * Cfg<HD>::kCtas * Cfg<HD>::kSlot * sizeof(float);
+    return (size_t)2 * Cfg<HD>::kCtas * (Cfg<HD>::kSlot + 2 * kRows) * sizeof(float);
 }
 
 }  // namespace
