@@ -10,6 +10,7 @@
 namespace {
 
 constexpr int kThreads = 128;   // four warps, each its own 16 tokens x 64 dimensions
+constexpr int kManyBlocks = 148 * 16;
 
 // Tiles of 16 tokens: sequence b has the slots [offsets[b] / 16 + 2 b,
 // offsets[b + 1] / 16 + 2 (b + 1)), at least as many as the records that its
@@ -45,129 +46,202 @@ G4_DEV bool find_tile(const Kv4View &c, int slot, Tile &t) {
     return true;
 }
 
-// Code + 8 of x for a group with scale s: x / s to the nearest integer, ties to
-// even, exactly. x * inv is within 2^-21 of x / s (|x / s| < 8), so only values
-// that close to a tie need the division, whose rounded quotient is a tie only
-// if the exact one is: (k + 1/2) s has 12 significant bits, so any other x is
-// further from it than half a step of the quotient.
-G4_DEV uint32_t code_of(float x, float s, float inv) {
-    const float t = x * inv;
-    float r = rintf(t);
-    if (fabsf(fabsf(t - r) - 0.5f) < 0x1p-18f) r = rintf(__fdiv_rn(x, s));
-    return (uint32_t)(int)(fminf(fmaxf(r, -7.0f), 7.0f) + 8.0f);
+// Codes + 8 of 8 values of a group with scale s, a nibble each: x / s to the nearest
+// integer, ties to even, exactly. x inv with one correction is x / s to within
+// 2^-22 of half a step, which decides every case: where x / s is a tie it is one of
+// fp32's values, and because (k + 1/2) s has 12 significant bits, any other x / s is
+// more than 1.004 half steps away from a tie. (Bf16 inputs often meet ties, so that
+// a division for those near one was taken by nearly every warp: 103 us for 32768
+// rows of 8 x 128.) Adding 1.5 2^23 + 8 rounds to an integer, ties to even because
+// the constant is even, whose low nibble is the code; the sum packs the nibbles.
+G4_DEV uint32_t pack8(const float *x, float s, float inv) {
+    constexpr float kMagic = 12582920.0f;                           // 0x4b400008
+    const uint64_t inv2 = pk(inv, inv), minus_s = pk(-s, -s), one = pk(1.0f, 1.0f), magic = pk(kMagic, kMagic);
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        const uint64_t v = pk(x[i], x[i + 1]), t = mul2(v, inv2);
+        const float2 y = upk(fma2(fma2(fma2(t, minus_s, v), inv2, t), one, magic));
+        w += __float_as_uint(y.x) << (4 * i);
+        w += __float_as_uint(y.y) << (4 * i + 4);
+    }
+    constexpr uint32_t kTop = 0x4b400000u;                          // what each value adds above its nibble
+    return w - (kTop + (kTop << 4) + (kTop << 8));                  // shifted by 12 and more it is 0 modulo 2^32
 }
 
 // Scale of a group from its largest absolute value (as bits, so that NaN and
-// infinity are the largest).
+// infinity are the largest) and its reciprocal to an ulp; inv 0: all codes are 0.
+// The quotient by 7 is the correctly rounded one (a product and one correction), and
+// rounding that to bf16 rounds the exact quotient: a bf16 tie times 7 has 12 bits.
 G4_DEV uint32_t scale_of(uint32_t amax, float &s, float &inv) {
-    uint32_t b;
-    if (amax >= 0x7f000000u) b = 0x7fc0u;                           // not finite, or >= 2^127
-    else if (amax < 0x0d800000u) b = 0u;                            // < 2^-100
-    else b = __bfloat16_as_ushort(__float2bfloat16_rn(__fdiv_rn(__uint_as_float(amax), 7.0f)));
+    constexpr float k7 = 0x1.24924ap-3f;                            // 1 / 7
+    const float a = __uint_as_float(amax), q = a * k7;
+    uint32_t b = __bfloat16_as_ushort(__float2bfloat16_rn(fmaf(fmaf(-7.0f, q, a), k7, q)));
     s = bf16_bits_f(b);
-    inv = (b == 0u || b == 0x7fc0u) ? 0.0f : __frcp_rn(s);
-    if (b == 0x7fc0u) s = 1.0f;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+    if (amax - 0x0d800000u >= 0x7f000000u - 0x0d800000u) {          // < 2^-100, or >= 2^127, or not finite
+        inv = 0.0f;
+        b = amax >= 0x7f000000u ? 0x7fc0u : 0u;
+    }
     return b;
 }
 
-template <int N>
-G4_DEV uint32_t abs_max(const float (&x)[N]) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < N; i++) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
-    return m;
-}
-
-G4_DEV uint32_t pack8(const float *x, float s, float inv, bool nan) {
-    uint32_t w = 0;
-#pragma unroll
-    for (int i = 0; i < 8; i++) w |= code_of(nan ? 0.0f : x[i], s, inv) << (4 * i);
-    return w;
-}
-
-// One warp per (tile, kv head, K or V, group): lane (g, t) = (lane / 4, lane % 4)
-// holds what the attention kernel's lane will read: for K the 16 dimensions 16 t
-// of tokens g and g + 8, for V the 8 dimensions 8 g of tokens 2t, 2t+1, 2t+8,
-// 2t+9. So a full tile's codes are one 512-byte store of the warp.
+// 8 values as they lie in memory, the largest |x| of them (as fp32 bits) and their
+// values; those of 16 bits are compared two at a time.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) k_kv4_write(Kv4View c, const T *k, long long k_stride, const T *v,
-                                                        long long v_stride, int parts) {
+struct Raw8 {
+    uint4 w[sizeof(T) / 2];
+    G4_DEV void load(const T *p) {
+        w[0] = reinterpret_cast<const uint4 *>(p)[0];
+        if constexpr (sizeof(T) == 4) w[1] = reinterpret_cast<const uint4 *>(p)[1];
+    }
+    G4_DEV void zero() {
+        w[0] = make_uint4(0, 0, 0, 0);
+        if constexpr (sizeof(T) == 4) w[1] = make_uint4(0, 0, 0, 0);
+    }
+};
+G4_DEV uint32_t max2(uint32_t a, uint32_t b) {
+    uint32_t y;
+    asm("max.u16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
+    return y;
+}
+G4_DEV uint32_t top(const Raw8<float> &r) {
+    constexpr uint32_t A = 0x7fffffffu;
+    return max(max(max(r.w[0].x & A, r.w[0].y & A), max(r.w[0].z & A, r.w[0].w & A)),
+               max(max(r.w[1].x & A, r.w[1].y & A), max(r.w[1].z & A, r.w[1].w & A)));
+}
+template <typename T>
+G4_DEV uint32_t top(const Raw8<T> &r) {
+    const uint32_t m2 = max2(max2(r.w[0].x & 0x7fff7fffu, r.w[0].y & 0x7fff7fffu),
+                             max2(r.w[0].z & 0x7fff7fffu, r.w[0].w & 0x7fff7fffu));
+    const uint32_t m = max(m2 & 0xffffu, m2 >> 16);
+    if constexpr (__is_same(T, __nv_bfloat16)) return m << 16;
+    else return __float_as_uint(__half2float(__ushort_as_half((unsigned short)m)));
+}
+G4_DEV void values(const Raw8<float> &r, float (&x)[8]) {
+    const uint32_t w[8] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w, r.w[1].x, r.w[1].y, r.w[1].z, r.w[1].w};
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = __uint_as_float(w[i]);
+}
+template <typename T>
+G4_DEV void values(const Raw8<T> &r, float (&x)[8]) {
+    const uint32_t w[4] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if constexpr (__is_same(T, __nv_bfloat16)) {
+            x[2 * i] = __uint_as_float(w[i] << 16);
+            x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        } else {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+            x[2 * i] = f.x;
+            x[2 * i + 1] = f.y;
+        }
+    }
+}
+template <typename T>
+G4_DEV uint32_t codes(const Raw8<T> &r, float s, float inv) {
+    float x[8];
+    values(r, x);
+    return inv == 0.0f ? 0x88888888u : pack8(x, s, inv);
+}
+
+// A warp takes units of a tile (kv head, group, K or V), `step` apart. Lane (g, t) =
+// (lane / 4, lane % 4) holds what the attention kernel's lane will read: for K the 16
+// dimensions 16 t of tokens g and g + 8, for V the 8 dimensions 8 g of tokens 2t,
+// 2t+1, 2t+8, 2t+9. So a full tile's codes are one 512-byte store of the warp.
+// (One unit per warp took 108 us for 32768 rows of 8 x 128 bf16: finding the tile
+// and its page is two dependent loads, a unit's data one.)
+// FULL: all 16 tokens of the record are rows.
+template <typename T, bool FULL>
+G4_DEV void write_units(const Kv4View &c, const T *k, long long k_stride, const T *v, long long v_stride,
+                        uint8_t *rec0, long long row0, int t0, int t1, int unit, int step) {
+    const int G = c.hd / kKv4Group, units = c.kv_heads * G * 2;
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const long long head_bytes = (long long)(17 * c.hd) << (c.page_shift - 4);
+    const T *k0 = k + (row0 + g) * k_stride + 16 * t, *v0 = v + (row0 + 2 * t) * v_stride + 8 * g;
+    auto in = [&](int tok) { return FULL || (tok >= t0 && tok < t1); };
+    for (; unit < units; unit += step) {
+        const int is_v = unit & 1, h = (unit >> 1) / G, grp = (unit >> 1) - h * G;
+        uint8_t *rec = rec0 + h * head_bytes;
+        uint16_t *ks = reinterpret_cast<uint16_t *>(rec + 16 * c.hd);
+        const int at = h * c.hd + grp * kKv4Group;
+        uint32_t w[4];
+        if (!is_v) {
+            Raw8<T> x[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if (in(g + 8 * (i >> 1))) x[i].load(k0 + at + (i >> 1) * 8 * k_stride + 8 * (i & 1));
+                else x[i].zero();
+            }
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                uint32_t m = max(top(x[2 * i]), top(x[2 * i + 1]));
+                m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                float s, inv;
+                const uint32_t b = scale_of(m, s, inv);
+                w[2 * i] = codes(x[2 * i], s, inv);
+                w[2 * i + 1] = codes(x[2 * i + 1], s, inv);
+                const int tok = g + 8 * i;
+                if (in(tok) && t == 0) ks[tok * G + grp] = (uint16_t)b;
+                if (!FULL && in(tok))
+                    *reinterpret_cast<uint2 *>(rec + grp * 512 + lane * 16 + 8 * i) =
+                        make_uint2(w[2 * i], w[2 * i + 1]);
+            }
+            if (FULL) *reinterpret_cast<uint4 *>(rec + grp * 512 + lane * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+        } else {
+            Raw8<T> x[4];
+            uint32_t m[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                if (in(2 * t + (j & 1) + 8 * (j >> 1))) x[j].load(v0 + at + ((j & 1) + 8 * (j >> 1)) * v_stride);
+                else x[j].zero();
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                m[j] = top(x[j]);
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) m[j] = max(m[j], __shfl_xor_sync(0xffffffffu, m[j], o));
+            }
+            // lane (g, t) makes the scale of its token j = g % 4 and hands it round
+            const uint32_t lo = g & 1 ? m[1] : m[0], hi = g & 1 ? m[3] : m[2];
+            float s1, inv1;
+            const uint32_t b = scale_of(g & 2 ? hi : lo, s1, inv1);
+            uint8_t *to = rec + 8 * c.hd + grp * 512 + lane * 16;
+            if (g < 4 && in(2 * t + (g & 1) + 8 * (g >> 1))) ks[16 * G + grp * 16 + t * 4 + g] = (uint16_t)b;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float s = __shfl_sync(0xffffffffu, s1, j * 4 + t), inv = __shfl_sync(0xffffffffu, inv1, j * 4 + t);
+                w[j] = codes(x[j], s, inv);
+                if (!FULL && in(2 * t + (j & 1) + 8 * (j >> 1))) *reinterpret_cast<uint32_t *>(to + 4 * j) = w[j];
+            }
+            if (FULL) *reinterpret_cast<uint4 *>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 8) k_kv4_write(Kv4View c, const T *k, long long k_stride, const T *v,
+                                                           long long v_stride, int parts) {
     griddep_wait();
-    const int slot = blockIdx.x / parts;
-    const int unit = (blockIdx.x % parts) * (kThreads / 32) + (threadIdx.x >> 5);
-    const int G = c.hd / kKv4Group;
-    if (unit >= c.kv_heads * G * 2) return;
+    const int slot = blockIdx.x / parts, step = parts * (kThreads / 32);
+    const int unit = (blockIdx.x - slot * parts) * (kThreads / 32) + (threadIdx.x >> 5);
+    if (unit >= c.kv_heads * (c.hd / kKv4Group) * 2) return;
     Tile tile;
     if (!find_tile(c, slot, tile) || tile.pos < 0) return;
-    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int is_v = unit & 1, grp = (unit >> 1) % G, h = (unit >> 1) / G;
-    uint8_t *rec = kv4_record(c, tile.seq, tile.pos, h);
-    if (!rec) return;
+    uint8_t *rec0 = kv4_record(c, tile.seq, tile.pos, 0);
+    if (!rec0) return;
     const int t0 = (int)(tile.pos & 15), t1 = t0 + tile.tokens;     // tokens of the record: [t0, t1)
     // first row of the record (may lie before the tensor; only rows of [t0, t1) are read)
     const long long row0 = (long long)tile.row - t0;
-    const bool full = tile.tokens == 16;
-    uint16_t *ks = reinterpret_cast<uint16_t *>(rec + 16 * c.hd);
-    if (!is_v) {
-        uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const int tok = g + 8 * i;
-            const bool mine = tok >= t0 && tok < t1;
-            float x[16];
-#pragma unroll
-            for (int j = 0; j < 16; j++) x[j] = 0.0f;
-            if (mine) {
-                const T *p = k + (row0 + tok) * k_stride + (long long)h * c.hd + grp * kKv4Group + 16 * t;
-                float y[8];
-                Kv4Vec<T>::load(p, y);
-#pragma unroll
-                for (int j = 0; j < 8; j++) x[j] = y[j];
-                Kv4Vec<T>::load(p + 8, y);
-#pragma unroll
-                for (int j = 0; j < 8; j++) x[8 + j] = y[j];
-            }
-            uint32_t m = abs_max(x);
-            m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-            m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-            float s, inv;
-            const uint32_t b = scale_of(m, s, inv);
-            w[2 * i] = pack8(x, s, inv, b == 0x7fc0u);
-            w[2 * i + 1] = pack8(x + 8, s, inv, b == 0x7fc0u);
-            if (mine && t == 0) ks[tok * G + grp] = (uint16_t)b;
-            if (mine && !full)
-                *reinterpret_cast<uint2 *>(rec + grp * 512 + lane * 16 + 8 * i) = make_uint2(w[2 * i], w[2 * i + 1]);
-        }
-        if (full) *reinterpret_cast<uint4 *>(rec + grp * 512 + lane * 16) = make_uint4(w[0], w[1], w[2], w[3]);
-    } else {
-        uint32_t w[4];
-        uint16_t *vs = ks + 16 * G + grp * 16 + t * 4;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int tok = 2 * t + (j & 1) + 8 * (j >> 1);
-            const bool mine = tok >= t0 && tok < t1;
-            float x[8];
-#pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = 0.0f;
-            if (mine) Kv4Vec<T>::load(v + (row0 + tok) * v_stride + (long long)h * c.hd + grp * kKv4Group + 8 * g, x);
-            uint32_t m = abs_max(x);
-#pragma unroll
-            for (int o = 4; o < 32; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-            float s, inv;
-            const uint32_t b = scale_of(m, s, inv);
-            w[j] = pack8(x, s, inv, b == 0x7fc0u);
-            if (mine && g == 0) vs[j] = (uint16_t)b;
-            if (mine && !full)
-                *reinterpret_cast<uint32_t *>(rec + 8 * c.hd + grp * 512 + lane * 16 + 4 * j) = w[j];
-        }
-        if (full)
-            *reinterpret_cast<uint4 *>(rec + 8 * c.hd + grp * 512 + lane * 16) = make_uint4(w[0], w[1], w[2], w[3]);
-    }
+    if (tile.tokens == 16) write_units<T, true>(c, k, k_stride, v, v_stride, rec0, row0, t0, t1, unit, step);
+    else write_units<T, false>(c, k, k_stride, v, v_stride, rec0, row0, t0, t1, unit, step);
 }
 
 G4_DEV void unpack8(uint32_t w, float s, float (&x)[8]) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = (float)((int)((w >> (4 * i)) & 15u) - 8) * s;
+    for (int i = 0; i < 8; i++)         // 2^23 + n, without a conversion
+        x[i] = (__uint_as_float(0x4b000000u | ((w >> (4 * i)) & 15u)) - 8388616.0f) * s;
 }
 
 // The mirror of k_kv4_write. Rows at negative positions or without a page read as 0.
@@ -175,44 +249,58 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads) k_kv4_read(Kv4View c, T *k, long long k_stride, T *v, long long v_stride,
                                                        int parts) {
     griddep_wait();
-    const int slot = blockIdx.x / parts;
-    const int unit = (blockIdx.x % parts) * (kThreads / 32) + (threadIdx.x >> 5);
-    const int G = c.hd / kKv4Group;
-    if (unit >= c.kv_heads * G * 2) return;
+    const int slot = blockIdx.x / parts, step = parts * (kThreads / 32);
+    const int G = c.hd / kKv4Group, units = c.kv_heads * G * 2;
+    int unit = (blockIdx.x - slot * parts) * (kThreads / 32) + (threadIdx.x >> 5);
+    if (unit >= units) return;
     Tile tile;
     if (!find_tile(c, slot, tile)) return;
+    const uint8_t *rec0 = tile.pos < 0 ? nullptr : kv4_record(c, tile.seq, tile.pos, 0);
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int is_v = unit & 1, grp = (unit >> 1) % G, h = (unit >> 1) / G;
-    const uint8_t *rec = tile.pos < 0 ? nullptr : kv4_record(c, tile.seq, tile.pos, h);
     const int t0 = (int)(tile.pos & 15), t1 = t0 + tile.tokens;
     const long long row0 = (long long)tile.row - t0;
-    const int code0 = is_v ? 8 * c.hd : 0;
-    uint4 q = make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);   // codes of 0
-    if (rec) q = *reinterpret_cast<const uint4 *>(rec + code0 + grp * 512 + lane * 16);
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-    const uint16_t *ks = reinterpret_cast<const uint16_t *>(rec + 16 * c.hd);
-    if (!is_v) {
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const int tok = g + 8 * i;
-            if (tok < t0 || tok >= t1) continue;
-            const float s = rec ? bf16_bits_f(ks[tok * G + grp]) : 0.0f;
-            T *p = k + (row0 + tok) * k_stride + (long long)h * c.hd + grp * kKv4Group + 16 * t;
-            float x[8];
-            unpack8(w[2 * i], s, x);
-            Kv4Vec<T>::store(p, x);
-            unpack8(w[2 * i + 1], s, x);
-            Kv4Vec<T>::store(p + 8, x);
+    const long long head_bytes = (long long)(17 * c.hd) << (c.page_shift - 4);
+    for (; unit < units; unit += step) {
+        const int is_v = unit & 1, h = (unit >> 1) / G, grp = (unit >> 1) - h * G;
+        uint4 q = make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);   // codes of 0
+        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (rec0) {
+            const uint8_t *rec = rec0 + h * head_bytes;
+            const uint16_t *ks = reinterpret_cast<const uint16_t *>(rec + 16 * c.hd);
+            q = *reinterpret_cast<const uint4 *>(rec + (is_v ? 8 * c.hd : 0) + grp * 512 + lane * 16);
+            if (is_v) {
+                const uint2 w = *reinterpret_cast<const uint2 *>(ks + 16 * G + grp * 16 + t * 4);
+                s[0] = bf16_bits_f(w.x & 0xffffu);
+                s[1] = bf16_bits_f(w.x >> 16);
+                s[2] = bf16_bits_f(w.y & 0xffffu);
+                s[3] = bf16_bits_f(w.y >> 16);
+            } else {
+                s[0] = bf16_bits_f(ks[g * G + grp]);
+                s[1] = bf16_bits_f(ks[(g + 8) * G + grp]);
+            }
         }
-    } else {
-        const uint16_t *vs = ks + 16 * G + grp * 16 + t * 4;
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+        const long long at = (long long)h * c.hd + grp * kKv4Group;
+        float x[8];
+        if (!is_v) {
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int tok = 2 * t + (j & 1) + 8 * (j >> 1);
-            if (tok < t0 || tok >= t1) continue;
-            float x[8];
-            unpack8(w[j], rec ? bf16_bits_f(vs[j]) : 0.0f, x);
-            Kv4Vec<T>::store(v + (row0 + tok) * v_stride + (long long)h * c.hd + grp * kKv4Group + 8 * g, x);
+            for (int i = 0; i < 2; i++) {
+                const int tok = g + 8 * i;
+                if (tok < t0 || tok >= t1) continue;
+                T *p = k + (row0 + tok) * k_stride + at + 16 * t;
+                unpack8(w[2 * i], s[i], x);
+                Kv4Vec<T>::store(p, x);
+                unpack8(w[2 * i + 1], s[i], x);
+                Kv4Vec<T>::store(p + 8, x);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int tok = 2 * t + (j & 1) + 8 * (j >> 1);
+                if (tok < t0 || tok >= t1) continue;
+                unpack8(w[j], s[j], x);
+                Kv4Vec<T>::store(v + (row0 + tok) * v_stride + at + 8 * g, x);
+            }
         }
     }
 }
@@ -271,10 +359,12 @@ bool aligned4(const void *p) { return ((uintptr_t)p & 3) == 0; }
 template <typename T>
 cudaError_t launch_move(bool write, const Kv4View &c, const void *k, long long ks, const void *v, long long vs,
                         cudaStream_t st) {
-    const int units = c.kv_heads * (c.hd / kKv4Group) * 2;
-    const int parts = (units + kThreads / 32 - 1) / (kThreads / 32);
-    // rows <= 2^22, n <= 2^16 and parts <= 1024: below 2^31
-    const unsigned blocks = (unsigned)((c.rows / kKv4Rec + 2 * c.n) * parts);
+    // Blocks per tile: few tiles are spread over the GPU (64 rows: a unit per warp), many
+    // keep their units together.
+    const int units = c.kv_heads * (c.hd / kKv4Group) * 2, most = (units + kThreads / 32 - 1) / (kThreads / 32);
+    const int slots = c.rows / kKv4Rec + 2 * c.n;
+    const int parts = slots * most <= kManyBlocks ? most : (kManyBlocks + slots - 1) / slots;
+    const unsigned blocks = (unsigned)slots * parts;
     if (write)
         return g4_launch(k_kv4_write<T>, dim3(blocks), dim3(kThreads), 0, st, true, c, (const T *)k, ks,
                          (const T *)v, vs, parts);
