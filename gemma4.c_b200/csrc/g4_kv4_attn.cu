@@ -472,7 +472,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kOcc) k_kv4_attn(const __gr
             for (int o = 1; o < 8; o <<= 1) rep += __shfl_xor_sync(0xffffffffu, rep, o);
             if (qr < kRows) {
                 if (qc == 0)
-                    row_scale[qr] = fabsf(p.scale) * kLog2e * __uint_as_float((uint32_t)(127 + 24 - 13 + e) << 23);
+                    row_scale[qr] = fmaxf(fabsf(p.scale) * kLog2e * __uint_as_float((uint32_t)(127 + 24 - 13 + e) << 23),
+                                          0x1p-120f);     // a scale of 0 still leaves -inf what it is
                 const int to = ((qc >> 3) * 2 + (qc & 1)) * 32 + qr * 4 + (qc >> 1 & 3);
                 qhi[to] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
                 if (HILO) qlo[to] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
@@ -805,13 +806,23 @@ size_t ws_bytes() {
 
 }  // namespace
 
-size_t g4_kv4_attention_ws(const Kv4View &c, int, int) {
+// Many query rows per sequence (64 and more of a kv head on average) go to the tcgen05
+// tiles of 128 rows, few to this file's tiles of 8.
+static bool many_rows(const Kv4View &c, int q_heads) {
+    return (long long)c.rows * (q_heads / c.kv_heads) >= 64ll * c.n;
+}
+
+size_t g4_kv4_attention_ws(const Kv4View &c, int, int q_heads) {
+    if (c.n == 0) return 16;
+    if (many_rows(c, q_heads)) return kv4_prompt_ws(c, q_heads);
     return c.hd == 64 ? ws_bytes<64>() : c.hd == 128 ? ws_bytes<128>() : c.hd == 256 ? ws_bytes<256>() : ws_bytes<512>();
 }
 
 cudaError_t g4_launch_kv4_attention(const Kv4View &c, int type, int q_heads, const void *q, long long q_stride,
                                     void *out, long long out_stride, float scale, int window, void *ws,
                                     cudaStream_t st) {
+    if (many_rows(c, q_heads))
+        return kv4_launch_prompt(c, type, q_heads, q, q_stride, out, out_stride, scale, window, ws, st);
     AttnP p;
     p.c = c;
     p.type = type;

@@ -1,0 +1,798 @@
+// g4_kv4_prompt.cu — attention over the paged 4-bit KV cache for many query rows
+// of a sequence (prompts, chunks): tcgen05 GEMMs on tiles of 128 rows x 64 keys.
+//
+// With many rows per key the two products dominate (4 x rows x keys x hd FLOP), so
+// they run on the 5th-generation tensor cores, and what would otherwise cost as
+// much, turning 4-bit codes into operands, is done once per 128 rows:
+//   S = Q K^T   fp16 operands in shared memory, fp32 accumulator in TMEM
+//   O += P V    P (fp16) in TMEM as the A operand, V^T in shared memory
+// Operands: a key or value c * scale has 11 significant bits (8 of the scale, 3 of
+// the code), so as fp16 it is exact once the largest scale of the keys in work is
+// brought to a fixed power of two (scales below 2^-9 of the largest lose bits that
+// are 2^-23 of the largest value). q is scaled per row by a power of two; an fp32 q
+// is split into high and low fp16 (22 bits; one fp16 holds a 16-bit q exactly), and so is
+// p for every type (one fp16 p, 11 bits, would show beside an fp16 output's own rounding).
+//
+// A CTA has one accumulator of 128 rows x 256 dimensions, all that TMEM holds beside
+// two S and two P tiles. 512 dimensions take a cluster of two CTAs, each with half
+// of the dimensions of q, K and V: they exchange their halves of S through
+// distributed shared memory, so that neither product is done twice.
+// Roles of the 13 warps: 0-3 softmax (thread = row = TMEM lane), 4-11 conversion (each
+// a record of the tile and some of its groups, the next tile's codes in flight in
+// registers), 12 the MMAs. S and P are double-buffered: while the softmax works on tile
+// j, the MMAs of S_{j+1} and of P_{j-1} V run and tile j + 1 is converted.
+#include <cuda_runtime.h>
+
+#include "g4_kv4.cuh"
+#include "g4_tc.cuh"
+
+namespace {
+
+constexpr int kM = 128;            // query rows of a tile
+constexpr int kT = 64;             // keys of a tile: 4 records
+constexpr int kSoftWarps = 4, kConvWarps = 8;
+constexpr int kThreads = (kSoftWarps + kConvWarps + 1) * 32;
+constexpr int kSms = 148;
+constexpr int kJoinThreads = 256;
+constexpr float kLog2e = 1.4426950408889634f;
+// p is 2^11 times too large, and may pass 1 by 2^4 before the outputs are rescaled: its
+// halves stay below 2^15, and small p keep 16 bits down to 2^-20, then steps of 2^-35
+// (with 2^6 and 2^8 an output that only keys of p = 1e-6 make was 1 % off).
+constexpr float kSlack = 4.0f, kUp = 11.0f;
+constexpr uint32_t kColS = 0, kColP = 128, kColO = 256;      // TMEM columns: 2 x 64, 2 x (32 + 32), 256
+
+template <int HD, bool HILO>
+struct Cfg {
+    static constexpr int kDc = HD > 256 ? 256 : HD;          // dimensions of a CTA
+    static constexpr int kCl = HD / kDc;                     // CTAs of a cluster
+    static constexpr int G = kDc / kKv4Group;
+    static constexpr int kQ = G * kM * 128;                  // one half of q: G tiles of 128 rows x 128 bytes
+    static constexpr int kK = G * kT * 128;
+    static constexpr int kV = kDc * 128;                     // V^T: rows are dimensions, 64 keys
+    static constexpr int kX = kCl > 1 ? kM * kT * 4 : 0;     // the other CTA's half of S
+    static constexpr int kSmem = kQ * (HILO ? 2 : 1) + kK + kV + kX + 1024;
+};
+
+struct PromptP {
+    Kv4View c;
+    int type;
+    unsigned group;                // query heads per kv head
+    int tokens;                    // per tile: 128 / group
+    int slots, splits;             // row tiles (an upper bound), key ranges of each
+    const void *q;
+    void *out;
+    long long q_stride, out_stride;
+    float scale;
+    int window;
+    float *parts, *stats;          // [slots][kv heads][splits][128][HD], [..][2][128]
+};
+
+G4_DEV float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+G4_DEV uint32_t pack_h(float lo, float hi) {
+    uint32_t y;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
+    return y;
+}
+G4_DEV float2 unpack_h(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2 *>(&w)); }
+G4_DEV uint32_t fma_h(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t y;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(y) : "r"(a), "r"(b), "r"(c));
+    return y;
+}
+G4_DEV uint32_t mul_h(uint32_t a, uint32_t b) {
+    uint32_t y;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
+    return y;
+}
+// 2^e as fp32, e in -126..127
+G4_DEV float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+G4_DEV void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+G4_DEV uint32_t rank_addr(uint32_t addr, uint32_t rank) {
+    uint32_t y;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(y) : "r"(addr), "r"(rank));
+    return y;
+}
+G4_DEV void remote_store4(uint32_t addr, float x, float y, float z, float w) {
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(x), "f"(y), "f"(z), "f"(w)
+                 : "memory");
+}
+G4_DEV void remote_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+G4_DEV bool wait_cluster(uint64_t *bar, uint32_t parity) {       // bounded, like mbar_wait
+    const uint64_t t0 = g4_globaltimer();
+    for (;;) {
+        uint32_t ok;
+        asm volatile(
+            "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+            " selp.u32 %0, 1, 0, p;\n}\n"
+            : "=r"(ok)
+            : "r"(smem_u32(bar)), "r"(parity)
+            : "memory");
+        if (ok) return true;
+        if (g4_globaltimer() - t0 > G4_WAIT_NS) return false;
+    }
+}
+G4_DEV void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+G4_DEV void mma_f16_ta(uint32_t tmem_d, uint32_t tmem_a, uint64_t db, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "r"(tmem_a), "l"(db), "r"(idesc), "r"((uint32_t)accumulate)
+        : "memory");
+}
+G4_DEV void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
+        "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
+        "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+        : "memory");
+}
+G4_DEV void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+G4_DEV void load8(const void *p, int type, long long i, float (&x)[8]) {
+    if (type == G4_TYPE_F32) Kv4Vec<float>::load((const float *)p + i, x);
+    else if (type == G4_TYPE_BF16) Kv4Vec<__nv_bfloat16>::load((const __nv_bfloat16 *)p + i, x);
+    else Kv4Vec<__half>::load((const __half *)p + i, x);
+}
+G4_DEV void store8(void *p, int type, long long i, const float (&x)[8]) {
+    if (type == G4_TYPE_F32) Kv4Vec<float>::store((float *)p + i, x);
+    else if (type == G4_TYPE_BF16) Kv4Vec<__nv_bfloat16>::store((__nv_bfloat16 *)p + i, x);
+    else Kv4Vec<__half>::store((__half *)p + i, x);
+}
+
+// ---- what a tile of rows sees ---------------------------------------------------
+// Row tiles: sequence b has the slots [offsets[b] / tokens + b, offsets[b + 1] / tokens
+// + b + 1), at least as many as its tiles of `tokens` tokens.
+struct Item {
+    int seq, row0, tok0, tokens;       // sequence, its first row, first token and tokens of the tile
+    long long pos0;                    // position of the sequence's first row
+    int see0, see1;                    // keys that some row sees (see1 < see0: none)
+    int all0, all1;                    // keys that every row sees
+};
+G4_DEV int slot_base(const PromptP &p, int b) { return kv4_offset(p.c, b) / p.tokens + b; }
+G4_DEV bool find_item(const PromptP &p, int slot, Item &it) {
+    int lo = 0, hi = p.c.n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (slot_base(p, mid) <= slot) lo = mid;
+        else hi = mid;
+    }
+    it.seq = lo;
+    it.row0 = kv4_offset(p.c, lo);
+    const int q = kv4_offset(p.c, lo + 1) - it.row0;
+    const int i = slot - slot_base(p, lo);
+    if (i < 0 || q <= 0 || i >= (q + p.tokens - 1) / p.tokens) return false;
+    it.tok0 = i * p.tokens;
+    it.tokens = min(p.tokens, q - it.tok0);
+    it.pos0 = p.c.start_pos[lo];
+    const long long cap = (long long)p.c.table_stride << p.c.page_shift, first = it.pos0 + it.tok0,
+                    last = first + it.tokens - 1;
+    it.see0 = p.window ? (int)min(max(first - p.window + 1, 0ll), cap) : 0;
+    it.see1 = (int)max(min(last, cap - 1), -1ll);
+    it.all0 = p.window ? (int)min(max(last - p.window + 1, 0ll), cap) : 0;
+    it.all1 = (int)max(min(first, cap - 1), -1ll);
+    return true;
+}
+// Key tiles of split s: [t0, t1)
+G4_DEV void tiles_of(const Item &it, int s, int splits, int &t0, int &t1) {
+    if (it.see1 < it.see0) {
+        t0 = t1 = 0;
+        return;
+    }
+    const int a = it.see0 / kT, n = it.see1 / kT + 1 - a;
+    t0 = a + (int)((long long)n * s / splits);
+    t1 = a + (int)((long long)n * (s + 1) / splits);
+}
+
+// Two codes (nibbles of the halves' bits m) times their scales: n 2^-21 or n 2^-17 (a
+// subnormal) times S, less 8 S: exact.
+G4_DEV uint32_t value2(uint32_t x, uint32_t mask, uint32_t s, uint32_t off) { return fma_h(x & mask, s, off); }
+// A scale for that: keys that no row of the tile sees may have larger ones than were
+// looked for (or anything); they only have to stay finite. NaN stays NaN.
+G4_DEV float bound(float f) { return f > 4080.0f ? 4080.0f : f; }
+constexpr uint32_t kLoMask = 0x00780078u, kHiMask = 0x07800780u;
+
+template <int HD, bool HILO>
+__global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constant__ PromptP p) {
+    using C = Cfg<HD, HILO>;
+    constexpr int G = C::G, HG = HD / kKv4Group, DC = C::kDc, CL = C::kCl;
+    constexpr int NB = G > 1 ? G / 2 : 1;                       // groups of a conversion warp
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t kfull, vfull, sfull[2], pfull[2], odone[2], xfull, xfree;
+    __shared__ uint32_t tmem_slot;
+    __shared__ float q_inv[kM];                                 // 1 / power of two of each row
+    __shared__ uint32_t k_top, v_top;                           // largest scales (bf16 bits) of the keys in work
+    __shared__ int missing[4][4];                               // [tile % 4][record]: tile + 1 if its page is missing
+    __shared__ int nan_tile[4];                                 // [tile % 4]: tile + 1 if a value of it is NaN
+    __shared__ uint32_t nan_keys[4][G][4];                      // [tile % 4][group][record]: (tile + 1) << 16 | keys
+    __shared__ int failed;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t rank = CL > 1 ? blockIdx.x % CL : 0;
+    uint8_t *base = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint8_t *qh = base, *ql = qh + (HILO ? C::kQ : 0), *kb = ql + C::kQ, *vb = kb + C::kK;
+    float4 *xb = reinterpret_cast<float4 *>(vb + C::kV);        // [16][128]: 4 keys x rows
+
+    griddep_wait();
+    const int id = blockIdx.x / CL;
+    const int split = id % p.splits, hs = id / p.splits, h = hs % p.c.kv_heads;
+    const int slot = p.slots - 1 - hs / p.c.kv_heads;           // the longest rows of a prompt first
+    Item it;
+    if (!find_item(p, slot, it)) return;                        // the same for the whole cluster
+    int t0, t1;
+    tiles_of(it, split, p.splits, t0, t1);
+    const int nt = t1 - t0;
+
+    if (tid == 0) {
+        mbar_init(&kfull, kConvWarps);
+        mbar_init(&vfull, kConvWarps);
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&sfull[i], 1);
+            mbar_init(&odone[i], 1);
+            mbar_init(&pfull[i], kSoftWarps);
+        }
+        mbar_init(&xfull, kSoftWarps);
+        mbar_init(&xfree, kSoftWarps);
+        k_top = v_top = 0;
+        failed = 0;
+    }
+    if (tid < 4) nan_tile[tid] = 0;
+    if (tid < 16) missing[tid >> 2][tid & 3] = 0;
+    if (tid < 16 * G) nan_keys[0][0][tid] = 0;
+    mbar_fence_init();
+    if (warp == kSoftWarps + kConvWarps) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_slot))
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    if constexpr (CL > 1) cluster_sync();
+    else __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    griddep_launch();
+
+    const int valid = it.tokens * (int)p.group;                 // rows of the tile: (token, head of the group)
+    auto q_row = [&](int r) {                                   // its place in q (or out), in elements, given the stride
+        const unsigned tok = (unsigned)r / p.group;
+        return (long long)(it.row0 + it.tok0 + (int)tok);
+    };
+    auto head_of = [&](int r) { return (long long)(h * p.group + (unsigned)r % p.group) * HD; };
+
+    // ---- prologue: query operands (softmax warps), largest scales (conversion warps) ----
+    if (warp < kSoftWarps) {
+        constexpr int LR = DC / 8 < 32 ? DC / 8 : 32;           // lanes of a row
+        constexpr int RP = 32 / LR;                             // rows of a pass
+        const int lr = lane / LR, ch = lane % LR;
+#pragma unroll 4
+        for (int r0 = warp * RP; r0 < kM; r0 += kSoftWarps * RP) {
+            const int r = r0 + lr;
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = 0.0f;
+            if (r < valid) load8(p.q, p.type, q_row(r) * p.q_stride + head_of(r) + rank * DC + ch * 8, x);
+            float mx = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) mx = fmaxf(mx, fabsf(x[i]));
+#pragma unroll
+            for (int o = 1; o < LR; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+            const int e = min(max((int)(__float_as_uint(mx) >> 23) - 127, -100), 115);
+            const float up = pow2(13 - e);
+            if (ch == 0) q_inv[r] = pow2(e - 13);
+            // dimensions in the order in which a word's codes come out: 0, 4, 1, 5, 2, 6, 3, 7
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float a = x[i] * up, b = x[i + 4] * up;
+                hi[i] = pack_h(a, b);
+                if (HILO) {
+                    const float2 f = unpack_h(hi[i]);
+                    lo[i] = pack_h(a - f.x, b - f.y);
+                }
+            }
+            const int to = (ch >> 3) * (kM * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
+            *reinterpret_cast<uint4 *>(qh + to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            if (HILO) *reinterpret_cast<uint4 *>(ql + to) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
+        fence_async();
+    } else if (warp < kSoftWarps + kConvWarps) {
+        uint32_t km = 0, vm = 0;
+        const int cw = warp - kSoftWarps, recs = nt * (kT / kKv4Rec);
+        for (int r0 = 0; r0 < recs; r0 += 32 * kConvWarps) {
+            // addresses of this warp's next 32 records, one per lane
+            const int mine = r0 + cw + lane * kConvWarps;
+            unsigned long long addr = 0;
+            if (mine < recs) addr = (unsigned long long)kv4_record(p.c, it.seq, (long long)t0 * kT + mine * 16, h);
+#pragma unroll 4
+            for (int k = 0; k < 32; k++) {
+                const int rec = r0 + cw + k * kConvWarps;
+                if (rec >= recs) break;
+                const uint8_t *src = (const uint8_t *)__shfl_sync(0xffffffffu, addr, k);
+                if (!src) continue;
+                const uint16_t *ks = reinterpret_cast<const uint16_t *>(src + 16 * HD), *vs = ks + 16 * HG;
+#pragma unroll
+                for (int i = 0; i < (16 * G + 31) / 32; i++) {
+                    const int x = i * 32 + lane;
+                    if (x < 16 * G) {
+                        const int kt = x / G, vt = 2 * (x >> 2 & 3) + (x & 1) + 8 * (x >> 1 & 1);   // tokens
+                        const int key = t0 * kT + rec * 16;
+                        const uint32_t a = ks[kt * HG + rank * G + x % G], b = vs[rank * G * 16 + x];
+                        if (key + kt >= it.see0 && key + kt <= it.see1 && a < 0x7f80u) km = max(km, a);
+                        if (key + vt >= it.see0 && key + vt <= it.see1 && b < 0x7f80u) vm = max(vm, b);
+                    }
+                }
+            }
+        }
+        km = __reduce_max_sync(0xffffffffu, km);
+        vm = __reduce_max_sync(0xffffffffu, vm);
+        if (lane == 0) {
+            atomicMax(&k_top, km);
+            atomicMax(&v_top, vm);
+        }
+    }
+    __syncthreads();
+    // scales times 2^ka (2^va) are at most 2^12; an operand is then the value times 2^(ka - 17)
+    const int ka = k_top ? min(max(11 - ((int)(k_top >> 7) - 127), -100), 113) : 0;
+    const int va = v_top ? min(max(11 - ((int)(v_top >> 7) - 127), -100), 113) : 0;
+
+    bool lost = false;                                          // a wait ran out: no more waits, the output is NaN
+    auto wait = [&](uint64_t *bar, int phase) {
+        if (!lost && !mbar_wait(bar, phase & 1, nullptr, 0)) {
+            lost = true;
+            failed = 1;
+        }
+    };
+
+    if (warp == kSoftWarps + kConvWarps) {
+        // ---- the MMAs ----
+        constexpr uint32_t kIdesc = (1u << 4) | ((uint32_t)(kM >> 4) << 24);       // fp16, fp16 -> fp32
+        constexpr uint32_t kIdS = kIdesc | ((uint32_t)(kT >> 3) << 17), kIdO = kIdesc | ((uint32_t)(DC >> 3) << 17);
+        if (lane == 0) {
+            for (int j = 0; j <= nt; j++) {
+                if (j < nt) {
+                    wait(&kfull, j);
+                    tc_fence_after();
+                    const uint32_t d = tmem + kColS + (j & 1) * kT;
+#pragma unroll
+                    for (int half = 0; half < (HILO ? 2 : 1); half++)
+#pragma unroll
+                        for (int i = 0; i < G * 4; i++)
+                            mma_f16(d, umma_desc((half ? ql : qh) + (i >> 2) * (kM * 128), (i & 3) * 32),
+                                    umma_desc(kb + (i >> 2) * (kT * 128), (i & 3) * 32), kIdS, half || i);
+                    mma_commit(&sfull[j & 1]);
+                }
+                if (j > 0) {
+                    const int i0 = j - 1, b = i0 & 1;
+                    wait(&vfull, i0);
+                    wait(&pfull[b], i0 >> 1);
+                    tc_fence_after();
+#pragma unroll
+                    for (int half = 0; half < 2; half++)
+#pragma unroll
+                        for (int i = 0; i < kT / 16; i++)
+                            mma_f16_ta(tmem + kColO, tmem + kColP + b * 64 + half * 32 + i * 8,
+                                       umma_desc(vb, i * 32), kIdO, i0 || half || i);
+                    mma_commit(&odone[b]);
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp >= kSoftWarps) {
+        // ---- conversion: this warp's record of each tile, its groups g0, g0 + 2, ... ----
+        const int cw = warp - kSoftWarps, rec = cw & 3, g0 = cw >> 2;
+        const bool busy = g0 < G;
+        const int g = lane >> 2, t = lane & 3;
+        const float kup = pow2(ka), vup = pow2(va);
+        auto record = [&](int j) -> const uint8_t * {
+            return j < nt ? kv4_record(p.c, it.seq, (long long)(t0 + j) * kT + rec * 16, h) : nullptr;
+        };
+        uint4 kc[NB], vc[NB];
+        uint32_t ks[NB];                                        // scales of keys g and g + 8
+        uint2 vs[NB];                                           // of keys 2t, 2t + 1, 2t + 8, 2t + 9
+        auto fetch = [&](const uint8_t *src) {
+#pragma unroll
+            for (int n = 0; n < NB; n++) {
+                const int gr = rank * G + g0 + 2 * n;
+                kc[n] = vc[n] = make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
+                ks[n] = 0;
+                vs[n] = make_uint2(0, 0);
+                if (src && busy) {
+                    const uint16_t *sc = reinterpret_cast<const uint16_t *>(src + 16 * HD);
+                    kc[n] = *reinterpret_cast<const uint4 *>(src + gr * 512 + lane * 16);
+                    vc[n] = *reinterpret_cast<const uint4 *>(src + 8 * HD + gr * 512 + lane * 16);
+                    ks[n] = (uint32_t)sc[g * HG + gr] | (uint32_t)sc[(g + 8) * HG + gr] << 16;
+                    vs[n] = *reinterpret_cast<const uint2 *>(sc + 16 * HG + gr * 16 + t * 4);
+                }
+            }
+        };
+        const uint8_t *src = record(0), *ahead = record(1);
+        fetch(src);
+        for (int j = 0; j < nt; j++) {
+            const uint4 kcj0 = kc[0], vcj0 = vc[0], kcj1 = kc[NB - 1], vcj1 = vc[NB - 1];
+            const uint32_t ksj[2] = {ks[0], ks[NB - 1]};
+            const uint2 vsj[2] = {vs[0], vs[NB - 1]};
+            const bool here = src != nullptr;
+            src = ahead;
+            fetch(src);                                         // the next tile's codes
+            ahead = record(j + 2);
+            if (!here && lane == 0) missing[j & 3][rec] = j + 1;
+            // NaN among the values: remembered by key, the operand is 0
+            uint2 vz[2] = {vsj[0], vsj[1]};
+            if (busy) {
+                bool bad = false;
+#pragma unroll
+                for (int n = 0; n < NB; n++) {
+                    const uint32_t w[2] = {vsj[n].x, vsj[n].y};
+#pragma unroll
+                    for (int i = 0; i < 2; i++) bad |= (w[i] & 0x7fffu) > 0x7f80u || (w[i] >> 16 & 0x7fffu) > 0x7f80u;
+                }
+                if (__any_sync(0xffffffffu, bad)) {
+#pragma unroll
+                    for (int n = 0; n < NB; n++) {
+                        uint32_t keys = 0;
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const uint32_t s = (i < 2 ? vsj[n].x : vsj[n].y) >> (16 * (i & 1)) & 0xffffu;
+                            if ((s & 0x7fffu) > 0x7f80u) {
+                                keys |= 1u << (2 * t + (i & 1) + 8 * (i >> 1));
+                                if (i < 2) vz[n].x &= ~(0xffffu << (16 * (i & 1)));
+                                else vz[n].y &= ~(0xffffu << (16 * (i & 1)));
+                            }
+                        }
+                        keys = __reduce_or_sync(0xffffffffu, keys);
+                        if (lane == 0) {
+                            nan_keys[j & 3][g0 + 2 * n][rec] = (uint32_t)(j + 1) << 16 | keys;
+                            nan_tile[j & 3] = j + 1;
+                        }
+                    }
+                }
+            }
+            // K rows are keys: a word's 8 dimensions are one 16-byte chunk
+            if (j > 0) wait(&sfull[(j - 1) & 1], (j - 1) >> 1);             // S_{j-1} has read the buffer
+            if (busy) {
+#pragma unroll
+                for (int n = 0; n < NB; n++) {
+                    const uint4 c4 = n ? kcj1 : kcj0;
+                    const uint32_t w[4] = {c4.x, c4.y, c4.z, c4.w};
+                    uint8_t *tile = kb + (g0 + 2 * n) * (kT * 128);
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        const float f = bound(__uint_as_float(i ? ksj[n] & 0xffff0000u : ksj[n] << 16) * kup);
+                        const uint32_t s = pack_h(f, f), s16 = pack_h(f * 16.0f, f * 16.0f),
+                                       off = mul_h(s, 0x84008400u);        // -2^-14 S
+                        const int row = rec * 16 + g + 8 * i;
+#pragma unroll
+                        for (int u = 0; u < 2; u++) {
+                            const uint32_t x = w[2 * i + u] << 3, y = w[2 * i + u] >> 5;
+                            const uint4 v4 = make_uint4(value2(x, kLoMask, s16, off), value2(x, kHiMask, s, off),
+                                                        value2(y, kLoMask, s16, off), value2(y, kHiMask, s, off));
+                            *reinterpret_cast<uint4 *>(tile + row * 128 + (((2 * t + u) ^ (row & 7)) << 4)) = v4;
+                        }
+                    }
+                }
+            }
+            fence_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&kfull);
+            // V^T rows are dimensions: a pair of keys is 4 bytes. Lane g starts with dimension
+            // 8 g + g % 8, so that the lanes of a store fall into different chunks.
+            if (j > 0) wait(&odone[(j - 1) & 1], (j - 1) >> 1);             // P_{j-1} V has read the buffer
+            if (busy) {
+#pragma unroll
+                for (int n = 0; n < NB; n++) {
+                    const uint4 c4 = n ? vcj1 : vcj0;
+                    const uint32_t rot = 4 * g;
+                    const uint32_t w0 = __funnelshift_r(c4.x, c4.x, rot), w1 = __funnelshift_r(c4.y, c4.y, rot),
+                                   w2 = __funnelshift_r(c4.z, c4.z, rot), w3 = __funnelshift_r(c4.w, c4.w, rot);
+#pragma unroll
+                    for (int pr = 0; pr < 2; pr++) {
+                        const uint32_t sw = pr ? vz[n].y : vz[n].x;
+                        const float f0 = bound(__uint_as_float(sw << 16) * vup),
+                                    f1 = bound(__uint_as_float(sw & 0xffff0000u) * vup);
+                        const uint32_t s = pack_h(f0, f1), s16 = pack_h(f0 * 16.0f, f1 * 16.0f),
+                                       off = mul_h(s, 0x84008400u);
+                        const int key = rec * 16 + 8 * pr + 2 * t;          // keys key, key + 1
+#pragma unroll
+                        for (int u = 0; u < 2; u++) {
+                            const uint32_t ab = __byte_perm(pr ? w2 : w0, pr ? w3 : w1, u ? 0x7632 : 0x5410);
+                            const uint32_t x = ab << 3, y = ab >> 5;
+                            const uint32_t v4[4] = {value2(x, kLoMask, s16, off), value2(x, kHiMask, s, off),
+                                                    value2(y, kLoMask, s16, off), value2(y, kHiMask, s, off)};
+#pragma unroll
+                            for (int i = 0; i < 4; i++) {
+                                const int d = (4 * u + i + g) & 7;          // dimension 8 g + d of the group
+                                const int row = (g0 + 2 * n) * 64 + 8 * g + d;
+                                *reinterpret_cast<uint32_t *>(vb + row * 128 + (((key >> 3) ^ d) << 4) +
+                                                              (key & 7) * 2) = v4[i];
+                            }
+                        }
+                    }
+                }
+            }
+            fence_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&vfull);
+        }
+    } else {
+        // ---- softmax: thread = row ----
+        const int r = tid;
+        const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
+        const long long pos = it.pos0 + it.tok0 + (unsigned)r / p.group;
+        const int cap = p.c.table_stride << p.c.page_shift;
+        const int my_hi = r < valid ? (int)max(min(pos, (long long)cap - 1), -1ll) : -1;
+        const int my_lo = p.window ? (int)min(max(pos - p.window + 1, 0ll), (long long)cap) : 0;
+        // the softmax scale's sign goes with q; a scale of 0 still leaves -inf what it is
+        const float cq = copysignf(q_inv[r] * pow2(min(17 - ka, 127)), p.scale),
+                    rs = fmaxf(fabsf(p.scale) * kLog2e, 0x1p-120f);
+        const uint32_t peer_x = CL > 1 ? rank_addr(smem_u32(xb), rank ^ 1) : 0;
+        const uint32_t peer_full = CL > 1 ? rank_addr(smem_u32(&xfull), rank ^ 1) : 0;
+        const uint32_t peer_free = CL > 1 ? rank_addr(smem_u32(&xfree), rank ^ 1) : 0;
+        float m = -INFINITY, l = 0.0f;
+        uint32_t nans = 0;                                      // groups with a NaN value that this row sees
+        for (int j = 0; j < nt; j++) {
+            const int b = j & 1;
+            wait(&sfull[b], j >> 1);
+            tc_fence_after();
+            float s[kT];
+            {
+                int v[32];
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    tmem_ld32(lanes + kColS + b * kT + i * 32, v);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int x = 0; x < 32; x++) s[i * 32 + x] = __int_as_float(v[x]) * cq;
+                }
+            }
+            if constexpr (CL > 1) {
+                // the halves of S: each CTA adds the other's to its own
+                if (j > 0 && !lost && !wait_cluster(&xfree, (j - 1) & 1)) lost = true, failed = 1;
+#pragma unroll
+                for (int i = 0; i < kT / 4; i++)
+                    remote_store4(peer_x + (uint32_t)(i * kM + r) * 16, s[4 * i], s[4 * i + 1], s[4 * i + 2],
+                                  s[4 * i + 3]);
+                asm volatile("fence.acq_rel.cluster;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) remote_arrive(peer_full);
+                if (!lost && !wait_cluster(&xfull, j & 1)) lost = true, failed = 1;
+#pragma unroll
+                for (int i = 0; i < kT / 4; i++) {
+                    const float4 x = xb[i * kM + r];
+                    s[4 * i] += x.x;
+                    s[4 * i + 1] += x.y;
+                    s[4 * i + 2] += x.z;
+                    s[4 * i + 3] += x.w;
+                }
+                __syncwarp();
+                if (lane == 0) remote_arrive(peer_free);
+            }
+            const int key0 = (t0 + j) * kT;
+            bool gap = false;
+#pragma unroll
+            for (int i = 0; i < 4; i++) gap |= missing[j & 3][i] == j + 1;
+            if (gap || key0 < it.all0 || key0 + kT - 1 > it.all1) {
+#pragma unroll
+                for (int i = 0; i < kT; i++)
+                    if (key0 + i < my_lo || key0 + i > my_hi || missing[j & 3][i >> 4] == j + 1) s[i] = -INFINITY;
+            }
+            if (nan_tile[j & 3] == j + 1) {
+                for (int gr = 0; gr < G; gr++)
+                    for (int rec = 0; rec < 4; rec++) {
+                        const uint32_t w = nan_keys[j & 3][gr][rec];
+                        if ((int)(w >> 16) == ((j + 1) & 0xffff))
+                            for (int i = 0; i < 16; i++) {
+                                const int key = key0 + rec * 16 + i;
+                                if ((w >> i & 1) && key >= my_lo && key <= my_hi) nans |= 1u << gr;
+                            }
+                    }
+            }
+            float mx = s[0];
+#pragma unroll
+            for (int i = 1; i < kT; i++) mx = fmaxf(mx, s[i]);
+            mx = mx * rs;
+            if (j > 1) wait(&odone[b], (j - 2) >> 1);           // P V of j - 2 has read this P
+            const bool grow = mx > m + kSlack;
+            if (__any_sync(0xffffffffu, grow)) {
+                const float mn = grow ? mx : m, al = mn == m ? 1.0f : ex2(m - mn);
+                m = mn;
+                l *= al;
+                if (j > 0) {
+                    wait(&odone[b ^ 1], (j - 1) >> 1);          // O is complete up to tile j - 1
+                    tc_fence_after();
+                    for (int c = 0; c < DC; c += 32) {
+                        int v[32];
+                        uint32_t u[32];
+                        tmem_ld32(lanes + kColO + c, v);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int x = 0; x < 32; x++) u[x] = __float_as_uint(__int_as_float(v[x]) * al);
+                        tmem_st32(lanes + kColO + c, u);
+                    }
+                    tmem_wait_st();
+                }
+            }
+            const float mref = (m == -INFINITY ? 0.0f : m) - kUp;
+            uint32_t ph[32], pl[32];
+            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < kT / 2; i++) {
+                const float a = ex2(fmaf(s[2 * i], rs, -mref)), c = ex2(fmaf(s[2 * i + 1], rs, -mref));
+                sum[i & 3] += a + c;
+                ph[i] = pack_h(a, c);
+                const float2 f = unpack_h(ph[i]);
+                pl[i] = pack_h(a - f.x, c - f.y);
+            }
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            tmem_st32(lanes + kColP + b * 64, ph);
+            tmem_st32(lanes + kColP + b * 64 + 32, pl);
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&pfull[b]);
+        }
+        if (nt > 0) wait(&odone[(nt - 1) & 1], (nt - 1) >> 1);
+        tc_fence_after();
+        if (failed) nans = 0xffffffffu;
+        // ---- output ----
+        const bool part = p.splits > 1;
+        const long long item = (long long)(slot * p.c.kv_heads + h) * p.splits + split;
+        const float fac = pow2(min(17 - va, 127)) * (part ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l);
+        if (part && rank == 0) {
+            p.stats[item * (2 * kM) + r] = m;
+            p.stats[item * (2 * kM) + kM + r] = l;
+        }
+#pragma unroll 1
+        for (int c = 0; c < DC; c += 32) {
+            int v[32];
+            if (nt > 0) {
+                tmem_ld32(lanes + kColO + c, v);
+                tmem_wait_ld();
+            } else {
+#pragma unroll
+                for (int x = 0; x < 32; x++) v[x] = 0;
+            }
+            const bool bad = nans >> (c / kKv4Group) & 1;
+#pragma unroll
+            for (int x = 0; x < 32; x += 8) {
+                float y[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) y[i] = bad ? NAN : __int_as_float(v[x + i]) * fac;
+                if (part) Kv4Vec<float>::store(p.parts + (item * kM + r) * HD + rank * DC + c + x, y);
+                else if (r < valid)
+                    store8(p.out, p.type, q_row(r) * p.out_stride + head_of(r) + rank * DC + c + x, y);
+            }
+        }
+    }
+    tc_fence_before();
+    if constexpr (CL > 1) cluster_sync();                       // the other CTA may still read or signal here
+    else __syncthreads();
+    if (warp == kSoftWarps + kConvWarps) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+}
+
+// Joins the key ranges of a row tile: block (slot x kv head, 8 rows).
+template <int HD>
+__global__ void __launch_bounds__(kJoinThreads) k_kv4_prompt_join(const __grid_constant__ PromptP p) {
+    __shared__ float f[32][8], inv[8];
+    const int tid = threadIdx.x, r0 = blockIdx.y * 8;
+    const int slot = blockIdx.x / p.c.kv_heads, h = blockIdx.x % p.c.kv_heads;
+    griddep_wait();
+    Item it;
+    if (!find_item(p, slot, it)) return;
+    const int valid = it.tokens * (int)p.group;
+    if (r0 >= valid) return;
+    const long long item = (long long)blockIdx.x * p.splits;
+    if (tid < 8) {
+        const float *st = p.stats + item * (2 * kM) + r0 + tid;
+        float m = -INFINITY, l = 0.0f;
+        for (int s = 0; s < p.splits; s++) m = fmaxf(m, st[s * (2 * kM)]);
+        const float ref = m == -INFINITY ? 0.0f : m;
+        for (int s = 0; s < p.splits; s++) {
+            const float x = ex2(st[s * (2 * kM)] - ref);
+            f[s][tid] = x;
+            l = fmaf(x, st[s * (2 * kM) + kM], l);
+        }
+        inv[tid] = l == 0.0f ? 0.0f : 1.0f / l;
+    }
+    __syncthreads();
+    for (int i = tid; i < HD; i += kJoinThreads) {              // 8 rows of HD / 8 pieces
+        const int r = i / (HD / 8), d = i % (HD / 8) * 8;
+        float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+        for (int s = 0; s < p.splits; s++) {
+            float y[8];
+            Kv4Vec<float>::load(p.parts + ((item + s) * kM + r0 + r) * HD + d, y);
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[j] = fmaf(f[s][r], y[j], x[j]);
+        }
+        if (r0 + r < valid) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[j] *= inv[r];
+            const unsigned tok = (unsigned)(r0 + r) / p.group;
+            store8(p.out, p.type,
+                   (long long)(it.row0 + it.tok0 + (int)tok) * p.out_stride +
+                       (long long)(h * p.group + (unsigned)(r0 + r) % p.group) * HD + d, x);
+        }
+    }
+}
+
+// Key ranges per row tile: enough for four rounds of the GPU's clusters when there are
+// few tiles, each of 8 key tiles or more. At most 32.
+void plan(const Kv4View &c, unsigned group, int *tokens, int *slots, int *splits) {
+    *tokens = kM / (int)group;
+    *slots = c.rows / *tokens + c.n;
+    const long long items = (long long)*slots * c.kv_heads, room = kSms / (c.hd > 256 ? 2 : 1);
+    const long long most = ((long long)c.table_stride << c.page_shift) / (8 * kT);
+    long long s = items >= 2 * room ? 1 : (4 * room + items - 1) / items;
+    s = s > most ? most : s;
+    *splits = s < 1 ? 1 : s > 32 ? 32 : (int)s;
+}
+
+template <int HD, bool HILO>
+cudaError_t launch_prompt(const PromptP &p, cudaStream_t st) {
+    using C = Cfg<HD, HILO>;
+    cudaError_t e = g4_smem_optin((const void *)k_kv4_prompt<HD, HILO>, C::kSmem);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)p.slots * p.c.kv_heads * p.splits * C::kCl);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = C::kSmem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = C::kCl;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = C::kCl > 1 ? 2 : 1;
+    e = cudaLaunchKernelEx(&cfg, k_kv4_prompt<HD, HILO>, p);
+    if (e != cudaSuccess || p.splits == 1) return e;
+    return g4_launch(k_kv4_prompt_join<HD>, dim3((unsigned)p.slots * p.c.kv_heads, kM / 8), dim3(kJoinThreads), 0, st,
+                     true, p);
+}
+
+template <int HD>
+cudaError_t launch_hd(const PromptP &p, cudaStream_t st) {
+    return p.type == G4_TYPE_F32 ? launch_prompt<HD, true>(p, st) : launch_prompt<HD, false>(p, st);
+}
+
+}  // namespace
+
+size_t kv4_prompt_ws(const Kv4View &c, int q_heads) {
+    int tokens, slots, splits;
+    plan(c, q_heads / c.kv_heads, &tokens, &slots, &splits);
+    return splits == 1 ? 16 : (size_t)slots * c.kv_heads * splits * kM * (c.hd + 2) * sizeof(float);
+}
+
+cudaError_t kv4_launch_prompt(const Kv4View &c, int type, int q_heads, const void *q, long long q_stride, void *out,
+                              long long out_stride, float scale, int window, void *ws, cudaStream_t st) {
+    PromptP p;
+    p.c = c;
+    p.type = type;
+    p.group = q_heads / c.kv_heads;
+    plan(c, p.group, &p.tokens, &p.slots, &p.splits);
+    p.q = q;
+    p.out = out;
+    p.q_stride = q_stride;
+    p.out_stride = out_stride;
+    p.scale = scale;
+    p.window = window;
+    p.parts = (float *)ws;
+    p.stats = p.parts + (size_t)p.slots * c.kv_heads * p.splits * kM * c.hd;
+    if (c.hd == 64) return launch_hd<64>(p, st);
+    if (c.hd == 128) return launch_hd<128>(p, st);
+    if (c.hd == 256) return launch_hd<256>(p, st);
+    return launch_hd<512>(p, st);
+}

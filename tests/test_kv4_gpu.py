@@ -297,6 +297,14 @@ def test_attention_prompts(g4, hd, heads, kv, name):
     check_attention(g4, s, heads, name, 1 / np.sqrt(hd), 100, rng)
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.1, 1e-30])
+def test_attention_scales(g4, scale):
+    """A softmax scale of 0 (every visible key alike), a negative one, a tiny one."""
+    for spans in ([(40, 1), (7, 2)], [(40, 70)]):
+        for hd, heads in ((64, 4), (512, 8)):
+            check_attention(g4, Setup(g4, spans, 1, hd, 32), heads, "f32", scale, 30, np.random.default_rng(hd))
+
+
 def test_attention_pages_missing(g4):
     """Keys on missing pages are not seen; a row with none of its pages gives 0."""
     s = Setup(g4, [(100, 1), (20, 3), (90, 40)], 1, 256, 16)
