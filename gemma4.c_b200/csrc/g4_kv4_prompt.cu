@@ -96,9 +96,12 @@ G4_DEV uint32_t rank_addr(uint32_t addr, uint32_t rank) {
     asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(y) : "r"(addr), "r"(rank));
     return y;
 }
-G4_DEV void remote_store4(uint32_t addr, float x, float y, float z, float w) {
-    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(x), "f"(y), "f"(z), "f"(w)
-                 : "memory");
+// 16 bytes into the other CTA's shared memory, counted on its barrier
+G4_DEV void remote_store4(uint32_t addr, float x, float y, float z, float w, uint32_t bar) {
+    asm volatile(
+        "st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(addr),
+        "f"(x), "f"(y), "f"(z), "f"(w), "r"(bar)
+        : "memory");
 }
 G4_DEV void remote_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
@@ -240,7 +243,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
             mbar_init(&odone[i], 1);
             mbar_init(&pfull[i], kSoftWarps);
         }
-        mbar_init(&xfull, kSoftWarps);
+        mbar_init(&xfull, 1);
         mbar_init(&xfree, kSoftWarps);
         k_top = v_top = 0;
         failed = 0;
@@ -318,22 +321,29 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
                 if (rec >= recs) break;
                 const uint8_t *src = (const uint8_t *)__shfl_sync(0xffffffffu, addr, k);
                 if (!src) continue;
-                const uint16_t *ks = reinterpret_cast<const uint16_t *>(src + 16 * HD), *vs = ks + 16 * HG;
+                // lanes 0-15: the K scales of a token, 16-31: G of the V scales
+                const bool is_v = lane >= 16;
+                const int i = lane & 15, key = t0 * kT + rec * 16;
+                const uint8_t *from = src + 16 * HD + (is_v ? 32 * HG + rank * (32 * G) + i * (2 * G)
+                                                            : i * (2 * HG) + rank * (2 * G));
+                uint32_t w[2] = {0, 0};
+                if constexpr (G == 4) {
+                    const uint2 x = *reinterpret_cast<const uint2 *>(from);
+                    w[0] = x.x;
+                    w[1] = x.y;
+                } else if constexpr (G == 2) w[0] = *reinterpret_cast<const uint32_t *>(from);
+                else w[0] = *reinterpret_cast<const uint16_t *>(from);
 #pragma unroll
-                for (int i = 0; i < (16 * G + 31) / 32; i++) {
-                    const int x = i * 32 + lane;
-                    if (x < 16 * G) {
-                        const int kt = x / G, vt = 2 * (x >> 2 & 3) + (x & 1) + 8 * (x >> 1 & 1);   // tokens
-                        const int key = t0 * kT + rec * 16;
-                        const uint32_t a = ks[kt * HG + rank * G + x % G], b = vs[rank * G * 16 + x];
-                        if (key + kt >= it.see0 && key + kt <= it.see1 && a < 0x7f80u) km = max(km, a);
-                        if (key + vt >= it.see0 && key + vt <= it.see1 && b < 0x7f80u) vm = max(vm, b);
-                    }
+                for (int x = 0; x < G; x++) {
+                    const uint32_t a = w[x / 2] >> (16 * (x & 1)) & 0xffffu;
+                    const int at = i * G + x, tok = is_v ? 2 * (at >> 2 & 3) + (at & 1) + 8 * (at >> 1 & 1) : i;
+                    if (key + tok >= it.see0 && key + tok <= it.see1 && a < 0x7f80u) km = max(km, a);
                 }
             }
         }
-        km = __reduce_max_sync(0xffffffffu, km);
-        vm = __reduce_max_sync(0xffffffffu, vm);
+        // K in the lower half of the warp, V in the upper one
+        vm = __reduce_max_sync(0xffffffffu, lane >= 16 ? km : 0);
+        km = __reduce_max_sync(0xffffffffu, lane >= 16 ? 0 : km);
         if (lane == 0) {
             atomicMax(&k_top, km);
             atomicMax(&v_top, vm);
@@ -395,78 +405,45 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
         auto record = [&](int j) -> const uint8_t * {
             return j < nt ? kv4_record(p.c, it.seq, (long long)(t0 + j) * kT + rec * 16, h) : nullptr;
         };
+        // K of a tile is converted before V of the tile before it, which waits for that tile's
+        // softmax; the codes after that are on their way in registers
         uint4 kc[NB], vc[NB];
         uint32_t ks[NB];                                        // scales of keys g and g + 8
-        uint2 vs[NB];                                           // of keys 2t, 2t + 1, 2t + 8, 2t + 9
-        auto fetch = [&](const uint8_t *src) {
+        uint2 vs[NB], vn[NB];                                   // of keys 2t, 2t + 1, 2t + 8, 2t + 9; the next tile's
+        auto fetch_k = [&](const uint8_t *src) {                // K codes, all scales
 #pragma unroll
             for (int n = 0; n < NB; n++) {
                 const int gr = rank * G + g0 + 2 * n;
-                kc[n] = vc[n] = make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
+                kc[n] = make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
                 ks[n] = 0;
-                vs[n] = make_uint2(0, 0);
+                vn[n] = make_uint2(0, 0);
                 if (src && busy) {
                     const uint16_t *sc = reinterpret_cast<const uint16_t *>(src + 16 * HD);
                     kc[n] = *reinterpret_cast<const uint4 *>(src + gr * 512 + lane * 16);
-                    vc[n] = *reinterpret_cast<const uint4 *>(src + 8 * HD + gr * 512 + lane * 16);
                     ks[n] = (uint32_t)sc[g * HG + gr] | (uint32_t)sc[(g + 8) * HG + gr] << 16;
-                    vs[n] = *reinterpret_cast<const uint2 *>(sc + 16 * HG + gr * 16 + t * 4);
+                    vn[n] = *reinterpret_cast<const uint2 *>(sc + 16 * HG + gr * 16 + t * 4);
                 }
             }
         };
-        const uint8_t *src = record(0), *ahead = record(1);
-        fetch(src);
-        for (int j = 0; j < nt; j++) {
-            const uint4 kcj0 = kc[0], vcj0 = vc[0], kcj1 = kc[NB - 1], vcj1 = vc[NB - 1];
-            const uint32_t ksj[2] = {ks[0], ks[NB - 1]};
-            const uint2 vsj[2] = {vs[0], vs[NB - 1]};
-            const bool here = src != nullptr;
-            src = ahead;
-            fetch(src);                                         // the next tile's codes
-            ahead = record(j + 2);
-            if (!here && lane == 0) missing[j & 3][rec] = j + 1;
-            // NaN among the values: remembered by key, the operand is 0
-            uint2 vz[2] = {vsj[0], vsj[1]};
-            if (busy) {
-                bool bad = false;
+        auto fetch_v = [&](const uint8_t *src) {
 #pragma unroll
-                for (int n = 0; n < NB; n++) {
-                    const uint32_t w[2] = {vsj[n].x, vsj[n].y};
-#pragma unroll
-                    for (int i = 0; i < 2; i++) bad |= (w[i] & 0x7fffu) > 0x7f80u || (w[i] >> 16 & 0x7fffu) > 0x7f80u;
-                }
-                if (__any_sync(0xffffffffu, bad)) {
-#pragma unroll
-                    for (int n = 0; n < NB; n++) {
-                        uint32_t keys = 0;
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const uint32_t s = (i < 2 ? vsj[n].x : vsj[n].y) >> (16 * (i & 1)) & 0xffffu;
-                            if ((s & 0x7fffu) > 0x7f80u) {
-                                keys |= 1u << (2 * t + (i & 1) + 8 * (i >> 1));
-                                if (i < 2) vz[n].x &= ~(0xffffu << (16 * (i & 1)));
-                                else vz[n].y &= ~(0xffffu << (16 * (i & 1)));
-                            }
-                        }
-                        keys = __reduce_or_sync(0xffffffffu, keys);
-                        if (lane == 0) {
-                            nan_keys[j & 3][g0 + 2 * n][rec] = (uint32_t)(j + 1) << 16 | keys;
-                            nan_tile[j & 3] = j + 1;
-                        }
-                    }
-                }
+            for (int n = 0; n < NB; n++) {
+                const int gr = rank * G + g0 + 2 * n;
+                vc[n] = make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
+                if (src && busy) vc[n] = *reinterpret_cast<const uint4 *>(src + 8 * HD + gr * 512 + lane * 16);
             }
-            // K rows are keys: a word's 8 dimensions are one 16-byte chunk
+        };
+        // K rows are keys: a word's 8 dimensions are one 16-byte chunk
+        auto convert_k = [&](int j) {
             if (j > 0) wait(&sfull[(j - 1) & 1], (j - 1) >> 1);             // S_{j-1} has read the buffer
             if (busy) {
 #pragma unroll
                 for (int n = 0; n < NB; n++) {
-                    const uint4 c4 = n ? kcj1 : kcj0;
-                    const uint32_t w[4] = {c4.x, c4.y, c4.z, c4.w};
+                    const uint32_t w[4] = {kc[n].x, kc[n].y, kc[n].z, kc[n].w};
                     uint8_t *tile = kb + (g0 + 2 * n) * (kT * 128);
 #pragma unroll
                     for (int i = 0; i < 2; i++) {
-                        const float f = bound(__uint_as_float(i ? ksj[n] & 0xffff0000u : ksj[n] << 16) * kup);
+                        const float f = bound(__uint_as_float(i ? ks[n] & 0xffff0000u : ks[n] << 16) * kup);
                         const uint32_t s = pack_h(f, f), s16 = pack_h(f * 16.0f, f * 16.0f),
                                        off = mul_h(s, 0x84008400u);        // -2^-14 S
                         const int row = rec * 16 + g + 8 * i;
@@ -483,19 +460,49 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
             fence_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(&kfull);
-            // V^T rows are dimensions: a pair of keys is 4 bytes. Lane g starts with dimension
-            // 8 g + g % 8, so that the lanes of a store fall into different chunks.
+        };
+        // NaN among the values of tile j: remembered by key, the operand is 0
+        auto find_nan = [&](int j) {
+            bool bad = false;
+#pragma unroll
+            for (int n = 0; n < NB; n++) {
+                const uint32_t w[2] = {vn[n].x, vn[n].y};
+#pragma unroll
+                for (int i = 0; i < 2; i++) bad |= (w[i] & 0x7fffu) > 0x7f80u || (w[i] >> 16 & 0x7fffu) > 0x7f80u;
+            }
+            if (!__any_sync(0xffffffffu, bad)) return;
+#pragma unroll
+            for (int n = 0; n < NB; n++) {
+                uint32_t keys = 0;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const uint32_t s = (i < 2 ? vn[n].x : vn[n].y) >> (16 * (i & 1)) & 0xffffu;
+                    if ((s & 0x7fffu) > 0x7f80u) {
+                        keys |= 1u << (2 * t + (i & 1) + 8 * (i >> 1));
+                        if (i < 2) vn[n].x &= ~(0xffffu << (16 * (i & 1)));
+                        else vn[n].y &= ~(0xffffu << (16 * (i & 1)));
+                    }
+                }
+                keys = __reduce_or_sync(0xffffffffu, keys);
+                if (lane == 0) {
+                    nan_keys[j & 3][g0 + 2 * n][rec] = (uint32_t)(j + 1) << 16 | keys;
+                    nan_tile[j & 3] = j + 1;
+                }
+            }
+        };
+        // V^T rows are dimensions: a pair of keys is 4 bytes. Lane g starts with dimension
+        // 8 g + g % 8, so that the lanes of a store fall into different chunks.
+        auto convert_v = [&](int j) {
             if (j > 0) wait(&odone[(j - 1) & 1], (j - 1) >> 1);             // P_{j-1} V has read the buffer
             if (busy) {
 #pragma unroll
                 for (int n = 0; n < NB; n++) {
-                    const uint4 c4 = n ? vcj1 : vcj0;
                     const uint32_t rot = 4 * g;
-                    const uint32_t w0 = __funnelshift_r(c4.x, c4.x, rot), w1 = __funnelshift_r(c4.y, c4.y, rot),
-                                   w2 = __funnelshift_r(c4.z, c4.z, rot), w3 = __funnelshift_r(c4.w, c4.w, rot);
+                    const uint32_t w0 = __funnelshift_r(vc[n].x, vc[n].x, rot), w1 = __funnelshift_r(vc[n].y, vc[n].y, rot),
+                                   w2 = __funnelshift_r(vc[n].z, vc[n].z, rot), w3 = __funnelshift_r(vc[n].w, vc[n].w, rot);
 #pragma unroll
                     for (int pr = 0; pr < 2; pr++) {
-                        const uint32_t sw = pr ? vz[n].y : vz[n].x;
+                        const uint32_t sw = pr ? vs[n].y : vs[n].x;
                         const float f0 = bound(__uint_as_float(sw << 16) * vup),
                                     f1 = bound(__uint_as_float(sw & 0xffff0000u) * vup);
                         const uint32_t s = pack_h(f0, f1), s16 = pack_h(f0 * 16.0f, f1 * 16.0f),
@@ -521,6 +528,40 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
             fence_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(&vfull);
+        };
+        // what the softmax has to know of tile j, before its K is passed on
+        auto note = [&](int j, const uint8_t *src) {
+            if (!src && lane == 0) missing[j & 3][rec] = j + 1;
+            if (busy) find_nan(j);
+        };
+        const uint8_t *r0 = record(0), *r1 = record(1), *r2 = record(2);    // of tiles j, j + 1, j + 2
+        fetch_k(r0);
+        fetch_v(r0);
+        if (nt > 0) {
+            note(0, r0);
+            convert_k(0);
+#pragma unroll
+            for (int n = 0; n < NB; n++) vs[n] = vn[n];
+            fetch_k(r1);
+        }
+        for (int j = 0; j < nt; j++) {
+            // in registers: V of tile j, K and the V scales of tile j + 1
+            uint2 next[NB];
+            if (j + 1 < nt) {
+                note(j + 1, r1);
+                convert_k(j + 1);
+#pragma unroll
+                for (int n = 0; n < NB; n++) next[n] = vn[n];
+                fetch_k(r2);
+            }
+            convert_v(j);
+            if (j + 1 < nt) {
+                fetch_v(r1);
+#pragma unroll
+                for (int n = 0; n < NB; n++) vs[n] = next[n];
+            }
+            r1 = r2;
+            r2 = record(j + 3);
         }
     } else {
         // ---- softmax: thread = row ----
@@ -559,10 +600,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
 #pragma unroll
                 for (int i = 0; i < kT / 4; i++)
                     remote_store4(peer_x + (uint32_t)(i * kM + r) * 16, s[4 * i], s[4 * i + 1], s[4 * i + 2],
-                                  s[4 * i + 3]);
-                asm volatile("fence.acq_rel.cluster;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) remote_arrive(peer_full);
+                                  s[4 * i + 3], peer_full);
+                if (tid == 0) mbar_arrive_expect_tx(&xfull, C::kX);
                 if (!lost && !wait_cluster(&xfull, j & 1)) lost = true, failed = 1;
 #pragma unroll
                 for (int i = 0; i < kT / 4; i++) {
