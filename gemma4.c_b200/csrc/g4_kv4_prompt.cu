@@ -17,9 +17,9 @@
 // two S and two P tiles. 512 dimensions take a cluster of two CTAs, each with half
 // of the dimensions of q, K and V: they exchange their halves of S through
 // distributed shared memory, so that neither product is done twice.
-// Roles of the 13 warps: 0-3 softmax (thread = row = TMEM lane), 4-11 conversion (each
-// a record of the tile and some of its groups, the next tile's codes in flight in
-// registers), 12 the MMAs. S and P are double-buffered: while the softmax works on tile
+// Roles of the 17 warps: 0-7 softmax (two threads per row = TMEM lane, 32 keys each),
+// 8-15 conversion (each a record of the tile and some of its groups, the next tile's
+// codes in flight in registers), 16 the MMAs. S and P are double-buffered: while the softmax works on tile
 // j, the MMAs of S_{j+1} and of P_{j-1} V run and tile j + 1 is converted.
 #include <cuda_runtime.h>
 
@@ -30,7 +30,8 @@ namespace {
 
 constexpr int kM = 128;            // query rows of a tile
 constexpr int kT = 64;             // keys of a tile: 4 records
-constexpr int kSoftWarps = 4, kConvWarps = 8;
+constexpr int kH = kT / 2;         // keys of a softmax thread
+constexpr int kSoftWarps = 8, kConvWarps = 8;
 constexpr int kThreads = (kSoftWarps + kConvWarps + 1) * 32;
 constexpr int kSms = 148;
 constexpr int kJoinThreads = 256;
@@ -50,7 +51,7 @@ struct Cfg {
     static constexpr int kK = G * kT * 128;
     static constexpr int kV = kDc * 128;                     // V^T: rows are dimensions, 64 keys
     static constexpr int kX = kCl > 1 ? kM * kT * 4 : 0;     // the other CTA's half of S
-    static constexpr int kSmem = kQ * (HILO ? 2 : 1) + kK + kV + kX + 1024;
+    static constexpr int kSmem = kQ * (HILO ? 2 : 1) + kK + kV + kX;
 };
 
 struct PromptP {
@@ -130,7 +131,7 @@ G4_DEV void mma_f16_ta(uint32_t tmem_d, uint32_t tmem_a, uint64_t db, uint32_t i
         "r"(tmem_a), "l"(db), "r"(idesc), "r"((uint32_t)accumulate)
         : "memory");
 }
-G4_DEV void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
+G4_DEV void tmem_st32(uint32_t taddr, const int (&v)[32]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
         "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
@@ -138,6 +139,14 @@ G4_DEV void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
         "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
         "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
         "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+        : "memory");
+}
+G4_DEV void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16};" ::"r"(taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
         : "memory");
 }
 G4_DEV void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -210,9 +219,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
     using C = Cfg<HD, HILO>;
     constexpr int G = C::G, HG = HD / kKv4Group, DC = C::kDc, CL = C::kCl;
     constexpr int NB = G > 1 ? G / 2 : 1;                       // groups of a conversion warp
-    extern __shared__ uint8_t smem_raw[];
+    extern __shared__ __align__(1024) uint8_t base[];          // tiles with the 128-byte swizzle
     __shared__ uint64_t kfull, vfull, sfull[2], pfull[2], odone[2], xfull, xfree;
     __shared__ uint32_t tmem_slot;
+    __shared__ float pair[2][2][kM];                            // between the two threads of a row
     __shared__ float q_inv[kM];                                 // 1 / power of two of each row
     __shared__ uint32_t k_top, v_top;                           // largest scales (bf16 bits) of the keys in work
     __shared__ int missing[4][4];                               // [tile % 4][record]: tile + 1 if its page is missing
@@ -221,7 +231,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
     __shared__ int failed;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t rank = CL > 1 ? blockIdx.x % CL : 0;
-    uint8_t *base = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint8_t *qh = base, *ql = qh + (HILO ? C::kQ : 0), *kb = ql + C::kQ, *vb = kb + C::kK;
     float4 *xb = reinterpret_cast<float4 *>(vb + C::kV);        // [16][128]: 4 keys x rows
 
@@ -271,43 +280,53 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
     };
     auto head_of = [&](int r) { return (long long)(h * p.group + (unsigned)r % p.group) * HD; };
 
-    // ---- prologue: query operands (softmax warps), largest scales (conversion warps) ----
-    if (warp < kSoftWarps) {
+    // ---- prologue: query operands (all but the MMA warp), largest scales (conversion warps) ----
+    if (warp < kSoftWarps + kConvWarps) {
         constexpr int LR = DC / 8 < 32 ? DC / 8 : 32;           // lanes of a row
-        constexpr int RP = 32 / LR;                             // rows of a pass
+        constexpr int RP = 32 / LR, RW = kM / (kSoftWarps + kConvWarps), NP = RW / RP;   // rows of a pass, of a warp
         const int lr = lane / LR, ch = lane % LR;
-#pragma unroll 4
-        for (int r0 = warp * RP; r0 < kM; r0 += kSoftWarps * RP) {
-            const int r = r0 + lr;
-            float x[8];
+#pragma unroll 1
+        for (int p0 = 0; p0 < NP; p0 += 2) {
+            float x[2][8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = 0.0f;
-            if (r < valid) load8(p.q, p.type, q_row(r) * p.q_stride + head_of(r) + rank * DC + ch * 8, x);
-            float mx = 0.0f;
+            for (int u = 0; u < 2; u++) {
+                const int r = warp * RW + (p0 + u) * RP + lr;
 #pragma unroll
-            for (int i = 0; i < 8; i++) mx = fmaxf(mx, fabsf(x[i]));
-#pragma unroll
-            for (int o = 1; o < LR; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-            const int e = min(max((int)(__float_as_uint(mx) >> 23) - 127, -100), 115);
-            const float up = pow2(13 - e);
-            if (ch == 0) q_inv[r] = pow2(e - 13);
-            // dimensions in the order in which a word's codes come out: 0, 4, 1, 5, 2, 6, 3, 7
-            uint32_t hi[4], lo[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float a = x[i] * up, b = x[i + 4] * up;
-                hi[i] = pack_h(a, b);
-                if (HILO) {
-                    const float2 f = unpack_h(hi[i]);
-                    lo[i] = pack_h(a - f.x, b - f.y);
-                }
+                for (int i = 0; i < 8; i++) x[u][i] = 0.0f;
+                if (p0 + u < NP && r < valid)
+                    load8(p.q, p.type, q_row(r) * p.q_stride + head_of(r) + rank * DC + ch * 8, x[u]);
             }
-            const int to = (ch >> 3) * (kM * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
-            *reinterpret_cast<uint4 *>(qh + to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            if (HILO) *reinterpret_cast<uint4 *>(ql + to) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                if (p0 + u >= NP) break;
+                const int r = warp * RW + (p0 + u) * RP + lr;
+                float mx = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8; i++) mx = fmaxf(mx, fabsf(x[u][i]));
+#pragma unroll
+                for (int o = 1; o < LR; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                const int e = min(max((int)(__float_as_uint(mx) >> 23) - 127, -100), 115);
+                const float up = pow2(13 - e);
+                if (ch == 0) q_inv[r] = pow2(e - 13);
+                // dimensions in the order in which a word's codes come out: 0, 4, 1, 5, 2, 6, 3, 7
+                uint32_t hi[4], lo[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float a = x[u][i] * up, b = x[u][i + 4] * up;
+                    hi[i] = pack_h(a, b);
+                    if (HILO) {
+                        const float2 f = unpack_h(hi[i]);
+                        lo[i] = pack_h(a - f.x, b - f.y);
+                    }
+                }
+                const int to = (ch >> 3) * (kM * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
+                *reinterpret_cast<uint4 *>(qh + to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                if (HILO) *reinterpret_cast<uint4 *>(ql + to) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            }
         }
         fence_async();
-    } else if (warp < kSoftWarps + kConvWarps) {
+    }
+    if (warp >= kSoftWarps && warp < kSoftWarps + kConvWarps) {
         uint32_t km = 0, vm = 0;
         const int cw = warp - kSoftWarps, recs = nt * (kT / kKv4Rec);
         for (int r0 = 0; r0 < recs; r0 += 32 * kConvWarps) {
@@ -564,9 +583,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
             r2 = record(j + 3);
         }
     } else {
-        // ---- softmax: thread = row ----
-        const int r = tid;
-        const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
+        // ---- softmax: threads (r, half) take keys 32 half .. + 31 of row r ----
+        const int quad = warp & 3, half = warp >> 2, r = quad * 32 + lane;
+        const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
         const long long pos = it.pos0 + it.tok0 + (unsigned)r / p.group;
         const int cap = p.c.table_stride << p.c.page_shift;
         const int my_hi = r < valid ? (int)max(min(pos, (long long)cap - 1), -1ll) : -1;
@@ -583,29 +602,27 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
             const int b = j & 1;
             wait(&sfull[b], j >> 1);
             tc_fence_after();
-            float s[kT];
+            float s[kH];
             {
-                int v[32];
+                int v[kH];
+                tmem_ld32(lanes + kColS + b * kT + half * kH, v);
+                tmem_wait_ld();
 #pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    tmem_ld32(lanes + kColS + b * kT + i * 32, v);
-                    tmem_wait_ld();
-#pragma unroll
-                    for (int x = 0; x < 32; x++) s[i * 32 + x] = __int_as_float(v[x]) * cq;
-                }
+                for (int x = 0; x < kH; x++) s[x] = __int_as_float(v[x]) * cq;
             }
             if constexpr (CL > 1) {
                 // the halves of S: each CTA adds the other's to its own
                 if (j > 0 && !lost && !wait_cluster(&xfree, (j - 1) & 1)) lost = true, failed = 1;
+                const int x0 = (half * (kH / 4)) * kM + r;
 #pragma unroll
-                for (int i = 0; i < kT / 4; i++)
-                    remote_store4(peer_x + (uint32_t)(i * kM + r) * 16, s[4 * i], s[4 * i + 1], s[4 * i + 2],
+                for (int i = 0; i < kH / 4; i++)
+                    remote_store4(peer_x + (uint32_t)(x0 + i * kM) * 16, s[4 * i], s[4 * i + 1], s[4 * i + 2],
                                   s[4 * i + 3], peer_full);
                 if (tid == 0) mbar_arrive_expect_tx(&xfull, C::kX);
                 if (!lost && !wait_cluster(&xfull, j & 1)) lost = true, failed = 1;
 #pragma unroll
-                for (int i = 0; i < kT / 4; i++) {
-                    const float4 x = xb[i * kM + r];
+                for (int i = 0; i < kH / 4; i++) {
+                    const float4 x = xb[x0 + i * kM];
                     s[4 * i] += x.x;
                     s[4 * i + 1] += x.y;
                     s[4 * i + 2] += x.z;
@@ -614,56 +631,59 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
                 __syncwarp();
                 if (lane == 0) remote_arrive(peer_free);
             }
-            const int key0 = (t0 + j) * kT;
-            bool gap = false;
+            const int key0 = (t0 + j) * kT + half * kH;
+            const bool gap0 = missing[j & 3][2 * half] == j + 1, gap1 = missing[j & 3][2 * half + 1] == j + 1;
+            if (gap0 || gap1 || key0 < it.all0 || key0 + kH - 1 > it.all1) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) gap |= missing[j & 3][i] == j + 1;
-            if (gap || key0 < it.all0 || key0 + kT - 1 > it.all1) {
-#pragma unroll
-                for (int i = 0; i < kT; i++)
-                    if (key0 + i < my_lo || key0 + i > my_hi || missing[j & 3][i >> 4] == j + 1) s[i] = -INFINITY;
+                for (int i = 0; i < kH; i++)
+                    if (key0 + i < my_lo || key0 + i > my_hi || (i < 16 ? gap0 : gap1)) s[i] = -INFINITY;
             }
             if (nan_tile[j & 3] == j + 1) {
                 for (int gr = 0; gr < G; gr++)
-                    for (int rec = 0; rec < 4; rec++) {
+                    for (int rec = 2 * half; rec < 2 * half + 2; rec++) {
                         const uint32_t w = nan_keys[j & 3][gr][rec];
                         if ((int)(w >> 16) == ((j + 1) & 0xffff))
                             for (int i = 0; i < 16; i++) {
-                                const int key = key0 + rec * 16 + i;
+                                const int key = (t0 + j) * kT + rec * 16 + i;
                                 if ((w >> i & 1) && key >= my_lo && key <= my_hi) nans |= 1u << gr;
                             }
                     }
             }
-            float mx = s[0];
+            float mx4[4];
 #pragma unroll
-            for (int i = 1; i < kT; i++) mx = fmaxf(mx, s[i]);
-            mx = mx * rs;
+            for (int i = 0; i < 4; i++) mx4[i] = s[i];
+#pragma unroll
+            for (int i = 4; i < kH; i++) mx4[i & 3] = fmaxf(mx4[i & 3], s[i]);
+            float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+            // the row's other half; the buffers alternate
+            pair[b][half][r] = mx;
+            bar_sync(1 + quad, 64);
+            mx = fmaxf(mx, pair[b][half ^ 1][r]) * rs;
             if (j > 1) wait(&odone[b], (j - 2) >> 1);           // P V of j - 2 has read this P
             const bool grow = mx > m + kSlack;
-            if (__any_sync(0xffffffffu, grow)) {
+            if (__any_sync(0xffffffffu, grow)) {                // the same in both warps of the rows
                 const float mn = grow ? mx : m, al = mn == m ? 1.0f : ex2(m - mn);
                 m = mn;
                 l *= al;
                 if (j > 0) {
                     wait(&odone[b ^ 1], (j - 1) >> 1);          // O is complete up to tile j - 1
                     tc_fence_after();
-                    for (int c = 0; c < DC; c += 32) {
+                    for (int c = half * (DC / 2); c < (half + 1) * (DC / 2); c += 32) {
                         int v[32];
-                        uint32_t u[32];
                         tmem_ld32(lanes + kColO + c, v);
                         tmem_wait_ld();
 #pragma unroll
-                        for (int x = 0; x < 32; x++) u[x] = __float_as_uint(__int_as_float(v[x]) * al);
-                        tmem_st32(lanes + kColO + c, u);
+                        for (int x = 0; x < 32; x++) v[x] = __float_as_int(__int_as_float(v[x]) * al);
+                        tmem_st32(lanes + kColO + c, v);
                     }
                     tmem_wait_st();
                 }
             }
             const float mref = (m == -INFINITY ? 0.0f : m) - kUp;
-            uint32_t ph[32], pl[32];
+            uint32_t ph[kH / 2], pl[kH / 2];
             float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int i = 0; i < kT / 2; i++) {
+            for (int i = 0; i < kH / 2; i++) {
                 const float a = ex2(fmaf(s[2 * i], rs, -mref)), c = ex2(fmaf(s[2 * i + 1], rs, -mref));
                 sum[i & 3] += a + c;
                 ph[i] = pack_h(a, c);
@@ -671,8 +691,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
                 pl[i] = pack_h(a - f.x, c - f.y);
             }
             l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            tmem_st32(lanes + kColP + b * 64, ph);
-            tmem_st32(lanes + kColP + b * 64 + 32, pl);
+            tmem_st16(lanes + kColP + b * 64 + half * 16, ph);
+            tmem_st16(lanes + kColP + b * 64 + 32 + half * 16, pl);
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
@@ -680,17 +700,21 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
         }
         if (nt > 0) wait(&odone[(nt - 1) & 1], (nt - 1) >> 1);
         tc_fence_after();
-        if (failed) nans = 0xffffffffu;
-        // ---- output ----
+        // ---- output: each thread of a row half of the dimensions ----
+        pair[0][half][r] = l;
+        pair[1][half][r] = __uint_as_float(failed ? 0xffffffffu : nans);
+        bar_sync(1 + quad, 64);
+        l += pair[0][half ^ 1][r];
+        nans |= __float_as_uint(pair[1][half][r]) | __float_as_uint(pair[1][half ^ 1][r]);
         const bool part = p.splits > 1;
         const long long item = (long long)(slot * p.c.kv_heads + h) * p.splits + split;
         const float fac = pow2(min(17 - va, 127)) * (part ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l);
-        if (part && rank == 0) {
+        if (part && rank == 0 && half == 0) {
             p.stats[item * (2 * kM) + r] = m;
             p.stats[item * (2 * kM) + kM + r] = l;
         }
 #pragma unroll 1
-        for (int c = 0; c < DC; c += 32) {
+        for (int c = half * (DC / 2); c < (half + 1) * (DC / 2); c += 32) {
             int v[32];
             if (nt > 0) {
                 tmem_ld32(lanes + kColO + c, v);
