@@ -20,7 +20,7 @@
 // Roles of the 17 warps: 0-7 softmax (two threads per row = TMEM lane, 32 keys each),
 // 8-15 conversion (each a record of the tile and some of its groups, the next tile's
 // codes in flight in registers), 16 the MMAs. S and P are double-buffered: while the softmax works on tile
-// j, the MMAs of S_{j+1} and of P_{j-1} V run and tile j + 1 is converted.
+// j, the MMAs of P_{j-1} V and S_{j+1} run and K of tile j + 2 and V of tile j are converted.
 #include <cuda_runtime.h>
 
 #include "g4_kv4.cuh"
@@ -36,10 +36,11 @@ constexpr int kThreads = (kSoftWarps + kConvWarps + 1) * 32;
 constexpr int kSms = 148;
 constexpr int kJoinThreads = 256;
 constexpr float kLog2e = 1.4426950408889634f;
-// p is 2^11 times too large, and may pass 1 by 2^4 before the outputs are rescaled: its
-// halves stay below 2^15, and small p keep 16 bits down to 2^-20, then steps of 2^-35
-// (with 2^6 and 2^8 an output that only keys of p = 1e-6 make was 1 % off).
-constexpr float kSlack = 4.0f, kUp = 11.0f;
+// The reference m of a row starts kHead above its first maximum and moves when the
+// maximum is kSlack above it, that is after growing by 2^7.9; p is 2^14 times too large.
+// So its halves stay below 65504, and p has steps of 2^-32 of the largest at most
+// (with a growth of 2^4 between rescalings two tiles in three had one, 0.8 us each).
+constexpr float kHead = 6.0f, kSlack = 1.9f, kUp = 14.0f;
 constexpr uint32_t kColS = 0, kColP = 128, kColO = 256;      // TMEM columns: 2 x 64, 2 x (32 + 32), 256
 
 template <int HD, bool HILO>
@@ -220,10 +221,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
     constexpr int G = C::G, HG = HD / kKv4Group, DC = C::kDc, CL = C::kCl;
     constexpr int NB = G > 1 ? G / 2 : 1;                       // groups of a conversion warp
     extern __shared__ __align__(1024) uint8_t base[];          // tiles with the 128-byte swizzle
-    __shared__ uint64_t kfull, vfull, sfull[2], pfull[2], odone[2], xfull, xfree;
+    __shared__ uint64_t kfull, vfull, sfull[2], pfull[2], odone[2];
+    __shared__ uint64_t xfull[kSoftWarps], xfree[kSoftWarps];   // a softmax warp and its like in the other CTA
     __shared__ uint32_t tmem_slot;
     __shared__ float pair[2][2][kM];                            // between the two threads of a row
-    __shared__ float q_inv[kM];                                 // 1 / power of two of each row
+    // 1 / power of two of each row's q: read by both threads of a row before they first meet,
+    // and so before tile 1 writes here
+    float *q_inv = pair[1][0];
     __shared__ uint32_t k_top, v_top;                           // largest scales (bf16 bits) of the keys in work
     __shared__ int missing[4][4];                               // [tile % 4][record]: tile + 1 if its page is missing
     __shared__ int nan_tile[4];                                 // [tile % 4]: tile + 1 if a value of it is NaN
@@ -252,8 +256,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
             mbar_init(&odone[i], 1);
             mbar_init(&pfull[i], kSoftWarps);
         }
-        mbar_init(&xfull, 1);
-        mbar_init(&xfree, kSoftWarps);
+        for (int i = 0; i < kSoftWarps; i++) {
+            mbar_init(&xfull[i], 1);
+            mbar_init(&xfree[i], 1);
+        }
         k_top = v_top = 0;
         failed = 0;
     }
@@ -386,9 +392,24 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
         constexpr uint32_t kIdesc = (1u << 4) | ((uint32_t)(kM >> 4) << 24);       // fp16, fp16 -> fp32
         constexpr uint32_t kIdS = kIdesc | ((uint32_t)(kT >> 3) << 17), kIdO = kIdesc | ((uint32_t)(DC >> 3) << 17);
         if (lane == 0) {
-            for (int j = 0; j <= nt; j++) {
-                if (j < nt) {
-                    wait(&kfull, j);
+            // S runs two tiles ahead of P V, so that the softmax of a tile never waits for an S
+            // that stands behind its own P V. (S_{j+2} overwrites S_j: P_j says that it was read.)
+            for (int j = -2; j < nt; j++) {
+                if (j >= 0) {
+                    const int b = j & 1;
+                    wait(&vfull, j);
+                    wait(&pfull[b], j >> 1);
+                    tc_fence_after();
+#pragma unroll
+                    for (int half = 0; half < 2; half++)
+#pragma unroll
+                        for (int i = 0; i < kT / 16; i++)
+                            mma_f16_ta(tmem + kColO, tmem + kColP + b * 64 + half * 32 + i * 8, umma_desc(vb, i * 32),
+                                       kIdO, j || half || i);
+                    mma_commit(&odone[b]);
+                }
+                if (j + 2 < nt) {
+                    wait(&kfull, j + 2);
                     tc_fence_after();
                     const uint32_t d = tmem + kColS + (j & 1) * kT;
 #pragma unroll
@@ -399,19 +420,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
                                     umma_desc(kb + (i >> 2) * (kT * 128), (i & 3) * 32), kIdS, half || i);
                     mma_commit(&sfull[j & 1]);
                 }
-                if (j > 0) {
-                    const int i0 = j - 1, b = i0 & 1;
-                    wait(&vfull, i0);
-                    wait(&pfull[b], i0 >> 1);
-                    tc_fence_after();
-#pragma unroll
-                    for (int half = 0; half < 2; half++)
-#pragma unroll
-                        for (int i = 0; i < kT / 16; i++)
-                            mma_f16_ta(tmem + kColO, tmem + kColP + b * 64 + half * 32 + i * 8,
-                                       umma_desc(vb, i * 32), kIdO, i0 || half || i);
-                    mma_commit(&odone[b]);
-                }
             }
         }
         __syncwarp();
@@ -421,11 +429,18 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
         const bool busy = g0 < G;
         const int g = lane >> 2, t = lane & 3;
         const float kup = pow2(ka), vup = pow2(va);
-        auto record = [&](int j) -> const uint8_t * {
-            return j < nt ? kv4_record(p.c, it.seq, (long long)(t0 + j) * kT + rec * 16, h) : nullptr;
+        // the page of this warp's record of tile j (loaded an iteration before it is looked at),
+        // and the record's address
+        const int *table = p.c.table + (long long)it.seq * p.c.table_stride;
+        auto page_of = [&](int j) -> int {
+            const int slot = ((t0 + j) * kT + rec * 16) >> p.c.page_shift;
+            return j < nt && slot < p.c.table_stride ? table[slot] : -1;
         };
-        // K of a tile is converted before V of the tile before it, which waits for that tile's
-        // softmax; the codes after that are on their way in registers
+        auto record = [&](int j, int page) -> const uint8_t * {
+            if ((unsigned)page >= (unsigned)p.c.num_pages) return nullptr;
+            const int in_page = ((t0 + j) * kT + rec * 16) & ((1 << p.c.page_shift) - 1);
+            return p.c.pages + page * p.c.page_bytes + (long long)(((h << p.c.page_shift) + in_page) >> 4) * (17 * HD);
+        };
         uint4 kc[NB], vc[NB];
         uint32_t ks[NB];                                        // scales of keys g and g + 8
         uint2 vs[NB], vn[NB];                                   // of keys 2t, 2t + 1, 2t + 8, 2t + 9; the next tile's
@@ -553,34 +568,45 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
             if (!src && lane == 0) missing[j & 3][rec] = j + 1;
             if (busy) find_nan(j);
         };
-        const uint8_t *r0 = record(0), *r1 = record(1), *r2 = record(2);    // of tiles j, j + 1, j + 2
-        fetch_k(r0);
-        fetch_v(r0);
-        if (nt > 0) {
-            note(0, r0);
-            convert_k(0);
+        // K is converted two tiles ahead of V, like the MMAs. In registers at the top of the
+        // loop: V of tile j; K and all scales of tile j + 2; the V scales of tile j + 1.
+        uint2 v1[NB];
+        auto keep = [&](uint2 (&to)[NB], const uint2 (&from)[NB]) {
 #pragma unroll
-            for (int n = 0; n < NB; n++) vs[n] = vn[n];
-            fetch_k(r1);
-        }
-        for (int j = 0; j < nt; j++) {
-            // in registers: V of tile j, K and the V scales of tile j + 1
-            uint2 next[NB];
-            if (j + 1 < nt) {
-                note(j + 1, r1);
-                convert_k(j + 1);
-#pragma unroll
-                for (int n = 0; n < NB; n++) next[n] = vn[n];
+            for (int n = 0; n < NB; n++) to[n] = from[n];
+        };
+        const uint8_t *r1 = record(1, page_of(1)), *r2 = record(2, page_of(2));       // of tiles j + 1, j + 2
+        int page = page_of(3);                                                        // of tile j + 3
+        {
+            const uint8_t *r0 = record(0, page_of(0));
+            fetch_k(r0);
+            fetch_v(r0);
+            if (nt > 0) {
+                note(0, r0);
+                convert_k(0);
+                keep(vs, vn);
+                fetch_k(r1);
+            }
+            if (nt > 1) {
+                note(1, r1);
+                convert_k(1);
+                keep(v1, vn);
                 fetch_k(r2);
             }
+        }
+        for (int j = 0; j < nt; j++) {
             convert_v(j);
-            if (j + 1 < nt) {
-                fetch_v(r1);
-#pragma unroll
-                for (int n = 0; n < NB; n++) vs[n] = next[n];
+            if (j + 1 < nt) fetch_v(r1);
+            keep(vs, v1);
+            if (j + 2 < nt) {
+                note(j + 2, r2);
+                convert_k(j + 2);
+                keep(v1, vn);
             }
             r1 = r2;
-            r2 = record(j + 3);
+            r2 = record(j + 3, page);
+            page = page_of(j + 4);
+            if (j + 3 < nt) fetch_k(r2);
         }
     } else {
         // ---- softmax: threads (r, half) take keys 32 half .. + 31 of row r ----
@@ -594,40 +620,55 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
         const float cq = copysignf(q_inv[r] * pow2(min(17 - ka, 127)), p.scale),
                     rs = fmaxf(fabsf(p.scale) * kLog2e, 0x1p-120f);
         const uint32_t peer_x = CL > 1 ? rank_addr(smem_u32(xb), rank ^ 1) : 0;
-        const uint32_t peer_full = CL > 1 ? rank_addr(smem_u32(&xfull), rank ^ 1) : 0;
-        const uint32_t peer_free = CL > 1 ? rank_addr(smem_u32(&xfree), rank ^ 1) : 0;
+        const uint32_t peer_full = CL > 1 ? rank_addr(smem_u32(&xfull[warp]), rank ^ 1) : 0;
+        const uint32_t peer_free = CL > 1 ? rank_addr(smem_u32(&xfree[warp]), rank ^ 1) : 0;
         float m = -INFINITY, l = 0.0f;
         uint32_t nans = 0;                                      // groups with a NaN value that this row sees
+        // this CTA's half of S of a tile to the other CTA: on its way while the tile before
+        // it is worked on
+        const int x0 = (half * (kH / 4)) * kM + r;
+        auto send = [&](int j) {
+            wait(&sfull[j & 1], j >> 1);
+            tc_fence_after();
+            if (j > 0 && !lost && !wait_cluster(&xfree[warp], (j - 1) & 1)) lost = true, failed = 1;
+#pragma unroll
+            for (int c = 0; c < kH; c += 16) {
+                int v[16];
+                tmem_ld16(lanes + kColS + (j & 1) * kT + half * kH + c, v);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    remote_store4(peer_x + (uint32_t)(x0 + (c / 4 + i) * kM) * 16, __int_as_float(v[4 * i]) * cq,
+                                  __int_as_float(v[4 * i + 1]) * cq, __int_as_float(v[4 * i + 2]) * cq,
+                                  __int_as_float(v[4 * i + 3]) * cq, peer_full);
+            }
+            if (lane == 0) mbar_arrive_expect_tx(&xfull[warp], C::kX / kSoftWarps);
+        };
+        if (CL > 1 && nt > 0) send(0);
         for (int j = 0; j < nt; j++) {
             const int b = j & 1;
-            wait(&sfull[b], j >> 1);
-            tc_fence_after();
             float s[kH];
+            if constexpr (CL == 1) {
+                wait(&sfull[b], j >> 1);
+                tc_fence_after();
+            } else if (!lost && !wait_cluster(&xfull[warp], j & 1)) lost = true, failed = 1;
             {
                 int v[kH];
                 tmem_ld32(lanes + kColS + b * kT + half * kH, v);
                 tmem_wait_ld();
 #pragma unroll
-                for (int x = 0; x < kH; x++) s[x] = __int_as_float(v[x]) * cq;
+                for (int i = 0; i < kH / 4; i++) {
+                    // the halves of S: each CTA adds the other's to its own. Both sums are the
+                    // same bits: the product with a power of two is exact.
+                    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if constexpr (CL > 1) x = xb[x0 + i * kM];
+                    s[4 * i] = fmaf(__int_as_float(v[4 * i]), cq, x.x);
+                    s[4 * i + 1] = fmaf(__int_as_float(v[4 * i + 1]), cq, x.y);
+                    s[4 * i + 2] = fmaf(__int_as_float(v[4 * i + 2]), cq, x.z);
+                    s[4 * i + 3] = fmaf(__int_as_float(v[4 * i + 3]), cq, x.w);
+                }
             }
             if constexpr (CL > 1) {
-                // the halves of S: each CTA adds the other's to its own
-                if (j > 0 && !lost && !wait_cluster(&xfree, (j - 1) & 1)) lost = true, failed = 1;
-                const int x0 = (half * (kH / 4)) * kM + r;
-#pragma unroll
-                for (int i = 0; i < kH / 4; i++)
-                    remote_store4(peer_x + (uint32_t)(x0 + i * kM) * 16, s[4 * i], s[4 * i + 1], s[4 * i + 2],
-                                  s[4 * i + 3], peer_full);
-                if (tid == 0) mbar_arrive_expect_tx(&xfull, C::kX);
-                if (!lost && !wait_cluster(&xfull, j & 1)) lost = true, failed = 1;
-#pragma unroll
-                for (int i = 0; i < kH / 4; i++) {
-                    const float4 x = xb[x0 + i * kM];
-                    s[4 * i] += x.x;
-                    s[4 * i + 1] += x.y;
-                    s[4 * i + 2] += x.z;
-                    s[4 * i + 3] += x.w;
-                }
                 __syncwarp();
                 if (lane == 0) remote_arrive(peer_free);
             }
@@ -659,10 +700,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
             pair[b][half][r] = mx;
             bar_sync(1 + quad, 64);
             mx = fmaxf(mx, pair[b][half ^ 1][r]) * rs;
-            if (j > 1) wait(&odone[b], (j - 2) >> 1);           // P V of j - 2 has read this P
             const bool grow = mx > m + kSlack;
             if (__any_sync(0xffffffffu, grow)) {                // the same in both warps of the rows
-                const float mn = grow ? mx : m, al = mn == m ? 1.0f : ex2(m - mn);
+                const float mn = grow ? mx + kHead : m, al = mn == m ? 1.0f : ex2(m - mn);
                 m = mn;
                 l *= al;
                 if (j > 0) {
@@ -679,6 +719,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
                     tmem_wait_st();
                 }
             }
+            if (CL > 1 && j + 1 < nt) send(j + 1);
             const float mref = (m == -INFINITY ? 0.0f : m) - kUp;
             uint32_t ph[kH / 2], pl[kH / 2];
             float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -691,6 +732,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
                 pl[i] = pack_h(a - f.x, c - f.y);
             }
             l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            if (j > 1) wait(&odone[b], (j - 2) >> 1);           // P V of j - 2 has read this P
             tmem_st16(lanes + kColP + b * 64 + half * 16, ph);
             tmem_st16(lanes + kColP + b * 64 + 32 + half * 16, pl);
             tmem_wait_st();
@@ -790,16 +832,23 @@ __global__ void __launch_bounds__(kJoinThreads) k_kv4_prompt_join(const __grid_c
     }
 }
 
-// Key ranges per row tile: enough for four rounds of the GPU's clusters when there are
-// few tiles, each of 8 key tiles or more. At most 32.
+// Key ranges per row tile, by the time of the rounds that the tiles then take: a key
+// tile costs 1, a range (its queries, scales and output) about 5. At most 32.
 void plan(const Kv4View &c, unsigned group, int *tokens, int *slots, int *splits) {
     *tokens = kM / (int)group;
     *slots = c.rows / *tokens + c.n;
-    const long long items = (long long)*slots * c.kv_heads, room = kSms / (c.hd > 256 ? 2 : 1);
-    const long long most = ((long long)c.table_stride << c.page_shift) / (8 * kT);
-    long long s = items >= 2 * room ? 1 : (4 * room + items - 1) / items;
-    s = s > most ? most : s;
-    *splits = s < 1 ? 1 : s > 32 ? 32 : (int)s;
+    const long long items = (long long)((c.rows + *tokens - 1) / *tokens) * c.kv_heads,
+                    room = kSms / (c.hd > 256 ? 2 : 1);
+    const int tiles = (int)((((long long)c.table_stride << c.page_shift) + kT - 1) / kT);
+    double best = 0.0;
+    *splits = 1;
+    for (int s = 1; s <= 32 && s <= tiles; s++) {
+        const double cost = (double)((items * s + room - 1) / room) * ((double)tiles / s + 5.0);
+        if (s == 1 || cost < 0.97 * best) {
+            best = cost;
+            *splits = s;
+        }
+    }
 }
 
 template <int HD, bool HILO>

@@ -66,7 +66,7 @@ def attention(q, keys, values, pos, scale, window):
     heads, hd = q.shape
     kv = keys.shape[1] if keys.ndim == 3 else 1
     out = np.zeros((heads, hd))
-    mag = np.zeros((heads, hd))          # sum of p |v|, and 2^-21 of the sum of |v| (see `tolerance`)
+    mag = np.zeros((heads, hd))          # sum of p |v|, and 2^-18 of the sum of |v| (see `tolerance`)
     first = max(0, pos - window + 1) if window else 0
     last = min(pos, keys.shape[0] - 1)
     if last < first:
@@ -83,7 +83,7 @@ def attention(q, keys, values, pos, scale, window):
         p = np.exp(s - s.max())
         p /= p.sum()
         out[h] = p @ v[:, j]
-        mag[h] = p @ np.abs(v[:, j]) + 2.0 ** -21 * np.abs(v[:, j]).sum(0)
+        mag[h] = p @ np.abs(v[:, j]) + 2.0 ** -18 * np.abs(v[:, j]).sum(0)
         # |q| against the largest code and the offset of the unsigned ones: 15 scales
         top = np.abs(k[:, j]).reshape(len(k), -1, GROUP).max(-1) / 7 * 15
         delta[h] = abs(scale) * (np.repeat(top, GROUP, -1) @ np.abs(q[h])).max()
@@ -96,9 +96,10 @@ def tolerance(out, mag, delta, n, eps):
     fp32 (8 * 2^-23), 8 groups are added: below 2^-19 of the sum of magnitudes
     `delta`; a probability moves by that much, its sum too (factor 2). Each
     probability keeps 16 bits (high and low parts: 2^-17), exp2 and its
-    argument 2^-20: together below 2^-15. In fp16 parts of 2^11 p the step is
-    2^-24 at least, an error of 2^-25 2^-11 = 2^-36 per key however small p is:
-    2^-15 of the 2^-21 sum |v| that `mag` holds. Sums over n keys add 2^-23 each.
+    argument 2^-20: together below 2^-15. In fp16 parts of 2^14 p, taken from a
+    reference up to 2^6 above the largest, the step is 2^-24 at least: an error of
+    2^-25 2^-14 2^6 = 2^-33 per key however small p is, 2^-15 of the 2^-18 sum |v|
+    that `mag` holds. Sums over n keys add 2^-23 each.
     The result is rounded once: eps / 2."""
     return mag * (2 * 2.0 ** -19 * delta[:, None] + 2.0 ** -15 + n * 2.0 ** -23) + np.abs(out) * eps / 2 * 1.01 + 1e-30
 
