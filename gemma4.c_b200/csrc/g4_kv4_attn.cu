@@ -218,7 +218,8 @@ template <int N>
 G4_DEV long long scan_total(const AttnP &p, Scan<N> &s, int per, long long &before, long long &mine) {
     const int tid = threadIdx.x, lane = tid & 31;
     mine = 0;
-    for (int b = tid * per; b < min((tid + 1) * per, p.c.n); b++) mine += work_of(p, seq_of(p, b));
+    // (bounded so that the sums stay in range for offsets that are not ascending as well)
+    for (int b = tid * per; b < min((tid + 1) * per, p.c.n); b++) mine = min(mine + work_of(p, seq_of(p, b)), 1ll << 50);
     long long inc = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -705,13 +706,21 @@ __global__ void __launch_bounds__(kJoinThreads) k_kv4_attn_join(const __grid_con
     const long long total = scan_total(p, scan, per, before, mine);
     const long long share = share_of(total, C::kCtas);
     const long long w = c * share;
-    if (w >= total) return;
+    // Every block waits for the parts, also one with nothing to join: this grid's end is
+    // what the next kernel of the stream goes by.
+    if (w >= total) {
+        griddep_wait();
+        return;
+    }
     find_work(p, scan, per, before, mine, w);
     const Seq s = seq_of(p, scan.seq);
     int item, inside;
     divide(scan.off, s.recs + kItemCost, item, inside);
     inside -= kItemCost;                               // records of the item before the cut
-    if (inside <= 0) return;                           // not a cut
+    if (inside <= 0) {                                 // not a cut
+        griddep_wait();
+        return;
+    }
     const int tile = item / p.c.kv_heads, h = item % p.c.kv_heads;
     // CTAs c0, c0 + 1, ... hold the parts: the item's records are the units from w - inside on
     const int ahead = (int)min(share, 1ll << 30);
@@ -806,10 +815,17 @@ size_t ws_bytes() {
 
 }  // namespace
 
-// Many query rows per sequence (64 and more of a kv head on average) go to the tcgen05
-// tiles of 128 rows, few to this file's tiles of 8.
+// Many query rows per sequence and kv head go to the tcgen05 tiles of 128 rows, few to
+// this file's tiles of 8, whose time grows with the rows while the other's starts at 30
+// (256 dimensions) to 50 us (512) for a context of 4000. Measured on either side, us here
+// and there: 16 sequences, 512 dimensions, 16 tokens x 8 heads on average 126 / 145, 33
+// tokens 234 / 209; 128 dimensions, 8 kv heads, 33 tokens x 4 heads 249 / 275, 65 tokens
+// 475 / 313; one sequence of 512 dimensions and one kv head, 64 tokens x 8 heads 47 / 54,
+// 128 tokens 80 / 60, of 256 dimensions 35 / 35 and 50 / 41. Fewer than four sequences and
+// heads of many dimensions leave the large tiles less to share out, hence their own bound.
 static bool many_rows(const Kv4View &c, int q_heads) {
-    return (long long)c.rows * (q_heads / c.kv_heads) >= 64ll * c.n;
+    const long long from = c.hd >= 256 && (long long)c.n * c.kv_heads < 4 ? 512 : 160;
+    return (long long)c.rows * (q_heads / c.kv_heads) >= from * c.n;
 }
 
 size_t g4_kv4_attention_ws(const Kv4View &c, int, int q_heads) {

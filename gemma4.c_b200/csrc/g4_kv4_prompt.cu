@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
     __shared__ uint32_t k_top, v_top;                           // largest scales (bf16 bits) of the keys in work
     __shared__ int missing[4][4];                               // [tile % 4][record]: tile + 1 if its page is missing
     __shared__ int nan_tile[4];                                 // [tile % 4]: tile + 1 if a value of it is NaN
-    __shared__ uint32_t nan_keys[4][G][4];                      // [tile % 4][group][record]: (tile + 1) << 16 | keys
+    __shared__ int2 nan_keys[4][G][4];                          // [tile % 4][group][record]: tile + 1, keys
     __shared__ int failed;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t rank = CL > 1 ? blockIdx.x % CL : 0;
@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
     }
     if (tid < 4) nan_tile[tid] = 0;
     if (tid < 16) missing[tid >> 2][tid & 3] = 0;
-    if (tid < 16 * G) nan_keys[0][0][tid] = 0;
+    if (tid < 16 * G) nan_keys[0][0][tid] = make_int2(0, 0);
     mbar_fence_init();
     if (warp == kSoftWarps + kConvWarps) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_slot))
@@ -519,7 +519,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
                 }
                 keys = __reduce_or_sync(0xffffffffu, keys);
                 if (lane == 0) {
-                    nan_keys[j & 3][g0 + 2 * n][rec] = (uint32_t)(j + 1) << 16 | keys;
+                    nan_keys[j & 3][g0 + 2 * n][rec] = make_int2(j + 1, (int)keys);
                     nan_tile[j & 3] = j + 1;
                 }
             }
@@ -682,11 +682,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
             if (nan_tile[j & 3] == j + 1) {
                 for (int gr = 0; gr < G; gr++)
                     for (int rec = 2 * half; rec < 2 * half + 2; rec++) {
-                        const uint32_t w = nan_keys[j & 3][gr][rec];
-                        if ((int)(w >> 16) == ((j + 1) & 0xffff))
+                        const int2 w = nan_keys[j & 3][gr][rec];
+                        if (w.x == j + 1)
                             for (int i = 0; i < 16; i++) {
                                 const int key = (t0 + j) * kT + rec * 16 + i;
-                                if ((w >> i & 1) && key >= my_lo && key <= my_hi) nans |= 1u << gr;
+                                if ((w.y >> i & 1) && key >= my_lo && key <= my_hi) nans |= 1u << gr;
                             }
                     }
             }
@@ -832,21 +832,35 @@ __global__ void __launch_bounds__(kJoinThreads) k_kv4_prompt_join(const __grid_c
     }
 }
 
-// Key ranges per row tile, by the time of the rounds that the tiles then take: a key
-// tile costs 1, a range (its queries, scales and output) about 5. At most 32.
-void plan(const Kv4View &c, unsigned group, int *tokens, int *slots, int *splits) {
-    *tokens = kM / (int)group;
-    *slots = c.rows / *tokens + c.n;
-    const long long items = (long long)((c.rows + *tokens - 1) / *tokens) * c.kv_heads,
-                    room = kSms / (c.hd > 256 ? 2 : 1);
-    const int tiles = (int)((((long long)c.table_stride << c.page_shift) + kT - 1) / kT);
+// Key ranges of a row tile that sees `tiles` key tiles, by the time of the rounds that
+// the row tiles then take: a key tile costs 1, a range (its queries, scales and output)
+// about 5. At most 32, and four rounds: more would not fill the GPU better, and the
+// partial outputs would grow.
+int ranges(const Kv4View &c, long long items, long long tiles) {
+    const long long room = kSms / (c.hd > 256 ? 2 : 1);
     double best = 0.0;
-    *splits = 1;
-    for (int s = 1; s <= 32 && s <= tiles; s++) {
+    int n = 1;
+    for (int s = 1; s <= 32 && s <= tiles && (s == 1 || items * s <= 4 * room); s++) {
         const double cost = (double)((items * s + room - 1) / room) * ((double)tiles / s + 5.0);
         if (s == 1 || cost < 0.97 * best) {
             best = cost;
-            *splits = s;
+            n = s;
+        }
+    }
+    return n;
+}
+// The workspace is sized without the window, which can only make the ranges fewer.
+void plan(const Kv4View &c, unsigned group, int window, int *tokens, int *slots, int *splits) {
+    *tokens = kM / (int)group;
+    *slots = c.rows / *tokens + c.n;
+    const long long items = (long long)((c.rows + *tokens - 1) / *tokens) * c.kv_heads,
+                    tiles = (((long long)c.table_stride << c.page_shift) + kT - 1) / kT;
+    *splits = ranges(c, items, tiles);
+    if (window) {
+        const long long seen = ((long long)window + *tokens - 1) / kT + 2;
+        if (seen < tiles) {
+            const int s = ranges(c, items, seen);
+            if (s < *splits) *splits = s;
         }
     }
 }
@@ -884,7 +898,7 @@ cudaError_t launch_hd(const PromptP &p, cudaStream_t st) {
 
 size_t kv4_prompt_ws(const Kv4View &c, int q_heads) {
     int tokens, slots, splits;
-    plan(c, q_heads / c.kv_heads, &tokens, &slots, &splits);
+    plan(c, q_heads / c.kv_heads, 0, &tokens, &slots, &splits);
     return splits == 1 ? 16 : (size_t)slots * c.kv_heads * splits * kM * (c.hd + 2) * sizeof(float);
 }
 
@@ -894,7 +908,7 @@ cudaError_t kv4_launch_prompt(const Kv4View &c, int type, int q_heads, const voi
     p.c = c;
     p.type = type;
     p.group = q_heads / c.kv_heads;
-    plan(c, p.group, &p.tokens, &p.slots, &p.splits);
+    plan(c, p.group, window, &p.tokens, &p.slots, &p.splits);
     p.q = q;
     p.out = out;
     p.q_stride = q_stride;

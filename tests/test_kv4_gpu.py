@@ -297,6 +297,85 @@ def test_attention_prompts(g4, hd, heads, kv, name):
     check_attention(g4, s, heads, name, 1 / np.sqrt(hd), 100, rng)
 
 
+PROMPT_SPANS = {
+    "whole": [(0, 150)],
+    "behind": [(333, 129)],
+    "mixed": [(0, 131), (700, 1), (61, 260), (-20, 90), (5, 0)],
+}
+
+
+@pytest.mark.parametrize("hd,kv,heads,page", [(64, 2, 8, 16), (64, 1, 64, 64), (128, 2, 10, 32), (128, 1, 3, 1024),
+                                              (256, 1, 8, 64), (256, 2, 8, 128), (512, 1, 8, 64), (512, 2, 10, 16)])
+@pytest.mark.parametrize("name", list(TYPES))
+@pytest.mark.parametrize("spans", list(PROMPT_SPANS))
+def test_prompt_tiles(g4, spans, name, hd, kv, heads, page):
+    """Row counts that go to the tiles of 128 rows: whole prompts, chunks inside
+    pages and tiles, sequences of one token among them, padding, tiles that the
+    heads of a group do not fill, windows."""
+    rng = np.random.default_rng(hd + heads)
+    s = Setup(g4, PROMPT_SPANS[spans], kv, hd, page)
+    check_attention(g4, s, heads, name, 1 / np.sqrt(hd), 0, rng, q_scale=2.0)
+    check_attention(g4, s, heads, name, -0.5 / np.sqrt(hd), 77, rng, pad=64)
+
+
+@pytest.mark.parametrize("hd,heads", [(64, 8), (256, 8), (512, 8)])
+def test_prompt_tiles_split(g4, hd, heads):
+    """Few row tiles over a long context: key ranges joined, with rows that see only some."""
+    rng = np.random.default_rng(hd)
+    check_attention(g4, Setup(g4, [(3000, 70)], 1, hd, 64), heads, "f32", 2 / np.sqrt(hd), 0, rng)
+    check_attention(g4, Setup(g4, [(3000, 70)], 1, hd, 64), heads, "bf16", 2 / np.sqrt(hd), 1100, rng)
+
+
+@pytest.mark.parametrize("hd", [64, 512])
+def test_prompt_tiles_pages_missing(g4, hd):
+    """Missing pages, among them all of a row tile's, and pages past the table."""
+    s = Setup(g4, [(100, 140), (20, 130), (90, 140), (0, 200)], 1, hd, 16)
+    s.table[0, 2] = -1
+    s.table[0, 6] = s.pages + 3
+    s.table[1, :] = -1
+    s.table[2, 3:9] = 2 ** 31 - 1
+    s.table[3, :5] = -9
+    s.upload()
+    check_attention(g4, s, 8, "f32", 0.1, 0, np.random.default_rng(5))
+
+
+@pytest.mark.parametrize("hd", [128, 512])
+def test_prompt_tiles_nan_and_infinity(g4, hd):
+    """A key or value that is not finite reaches the rows that see it (a value: the
+    dimensions of its group), and no other row, though they share its tile."""
+    s = Setup(g4, [(0, 200)], 1, hd, 64)
+    rng = np.random.default_rng(7)
+    k, v = tensors(rng, 200, 1, hd, torch.float32), tensors(rng, 200, 1, hd, torch.float32)
+    v[33, 0, 70] = float("nan")
+    k[150, 0, 3] = float("inf")
+    s.write(k, v, 0)
+    q = tensors(rng, 200, 8, hd, torch.float32)
+    q[20, 3, 5] = float("inf")
+    for window in (0, 60):
+        out = torch.empty_like(q)
+        s.attend(q, out, 0, 0.1, window)
+        for row in range(200):
+            bad = torch.zeros((8, hd), dtype=torch.bool, device="cuda:0")
+            if 33 <= row and (not window or row < 33 + window):
+                bad[:, 64:128] = True
+            if row >= 150:                              # the window still holds it
+                bad[:] = True
+            if row == 20:
+                bad[3] = True
+            assert torch.equal(torch.isnan(out[row]), bad), row
+
+
+def test_prompt_tiles_deterministic(g4):
+    rng = np.random.default_rng(3)
+    s = Setup(g4, [(900, 200)], 1, 512, 64)
+    q, out = check_attention(g4, s, 8, "f32", 0.1, 0, rng)
+    for fill in (0, 0x7F):
+        n = g4.kv4_attention_workspace(s.cache, s.batch, 0, 8)
+        again = torch.empty_like(out)
+        s.attend(q, again, 0, 0.1, 0, ws=torch.full((n,), fill, dtype=torch.uint8, device="cuda:0"))
+        assert torch.equal(out, again)
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.1, 1e-30])
 def test_attention_scales(g4, scale):
     """A softmax scale of 0 (every visible key alike), a negative one, a tiny one."""
