@@ -8,8 +8,8 @@
 //   O += P V    P (fp16) in TMEM as the A operand, V^T in shared memory
 // Operands: a key or value c * scale has 11 significant bits (8 of the scale, 3 of
 // the code), so as fp16 it is exact once the largest scale of the keys in work is
-// brought to a fixed power of two (scales below 2^-9 of the largest lose bits that
-// are 2^-23 of the largest value). q is scaled per row by a power of two; an fp32 q
+// brought to a fixed power of two (of scales below 2^-11 of the largest, bits are lost
+// that are 2^-20 of the largest value at most). q is scaled per row by a power of two; an fp32 q
 // is split into high and low fp16 (22 bits; one fp16 holds a 16-bit q exactly), and so is
 // p for every type (one fp16 p, 11 bits, would show beside an fp16 output's own rounding).
 //
@@ -211,8 +211,9 @@ G4_DEV void tiles_of(const Item &it, int s, int splits, int &t0, int &t1) {
 // subnormal) times S, less 8 S: exact.
 G4_DEV uint32_t value2(uint32_t x, uint32_t mask, uint32_t s, uint32_t off) { return fma_h(x & mask, s, off); }
 // A scale for that: keys that no row of the tile sees may have larger ones than were
-// looked for (or anything); they only have to stay finite. NaN stays NaN.
-G4_DEV float bound(float f) { return f > 4080.0f ? 4080.0f : f; }
+// looked for, or whatever an unwritten slot holds; they only have to stay finite (an
+// operand of 0 times infinity is NaN). NaN stays NaN.
+G4_DEV float bound(float f) { return f > 4080.0f ? 4080.0f : f < -4080.0f ? -4080.0f : f; }
 constexpr uint32_t kLoMask = 0x00780078u, kHiMask = 0x07800780u;
 
 template <int HD, bool HILO>

@@ -326,6 +326,13 @@ def test_prompt_tiles_split(g4, hd, heads):
     check_attention(g4, Setup(g4, [(3000, 70)], 1, hd, 64), heads, "bf16", 2 / np.sqrt(hd), 1100, rng)
 
 
+def test_prompt_tiles_window_needs_no_more_workspace(g4):
+    """The workspace is asked for without the window: every window fits into it."""
+    s = Setup(g4, [(0, 150)], 1, 256, 16, stride=4096)
+    for window in (1, 16, 64, 500, 20000, 2 ** 31 - 1):
+        check_attention(g4, s, 8, "bf16", 0.1, window, np.random.default_rng(window))
+
+
 @pytest.mark.parametrize("hd", [64, 512])
 def test_prompt_tiles_pages_missing(g4, hd):
     """Missing pages, among them all of a row tile's, and pages past the table."""
@@ -376,6 +383,35 @@ def test_prompt_tiles_deterministic(g4):
         assert torch.equal(out, again)
 
 
+@pytest.mark.parametrize("hd", [64, 512])
+@pytest.mark.parametrize("span", [(0, 200), (198, 2)])
+def test_attention_value_ranges(g4, hd, span):
+    """Keys and values whose sizes differ by 2^20. The tiles of 128 rows hold them as fp16
+    beside the largest that the tile sees, S in 2^11..2^12 a scale of it: an operand
+    c S 2^-17 is rounded twice (its offset 8 S too) by 2^-25 at most, that is c S by 2^-7,
+    and the largest value is 7 * 2^11 at least: 2^-7 / (7 * 2^11) < 2^-20 of it."""
+    rng = np.random.default_rng(hd)
+    s = Setup(g4, [(0, 200)], 1, hd, 64)
+    size = torch.exp2(-torch.from_numpy(rng.integers(0, 15, 200).astype(np.float32)))
+    size[180] = 64.0                                    # the first 180 rows do not see it
+    k, v = (tensors(rng, 200, 1, hd, torch.float32) * size.to("cuda:0")[:, None, None] for _ in range(2))
+    s.write(k, v, 0)
+    ks, vs = ref.stored(as64(k)), ref.stored(as64(v))
+    s.spans, s.offsets, s.rows = [span], np.array([0, span[1]], np.int32), span[1]
+    s.upload()
+    q = tensors(rng, span[1], 8, hd, torch.float32)
+    out = torch.empty_like(q)
+    s.attend(q, out, 0, 0.1, 0)
+    q64, got = as64(q), as64(out)
+    for row in range(span[1]):
+        want, mag, delta, n = ref.attention(q64[row], ks, vs, span[0] + row, 0.1, 0)
+        tol = ref.tolerance(want, mag, delta, n, 2.0 ** -23)
+        if span[1] > 2:
+            moved = 2 * 0.1 * 2.0 ** -20 * np.abs(ks).max() * np.abs(q64[row]).sum(-1)
+            tol = tol + mag * moved[:, None] + 2.0 ** -20 * np.abs(vs).max()
+        assert (np.abs(got[row] - want) <= tol).all(), row
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.1, 1e-30])
 def test_attention_scales(g4, scale):
     """A softmax scale of 0 (every visible key alike), a negative one, a tiny one."""
@@ -400,6 +436,15 @@ def test_attention_unwritten_neighbours(g4):
     for hd in (64, 512):
         s = Setup(g4, [(0, 1), (16, 1), (40, 2)], 1, hd, 64, fill=0xFF)
         check_attention(g4, s, 8, "f32", 0.1, 0, np.random.default_rng(6))
+
+
+@pytest.mark.parametrize("bits", [0x7F80, 0xFF80, 0x7F7F, 0xFF7F, 0xFFC0, 0x8001])
+def test_attention_unwritten_scales(g4, bits):
+    """Behind the last token scales of infinity, of the largest values, negative ones: never seen."""
+    for hd in (64, 256, 512):
+        for spans in ([(16, 1), (40, 2)], [(40, 70)], [(0, 150), (3, 9)]):
+            fill = np.tile(np.array([bits], np.uint16).view(np.uint8), 17 * hd // 2)
+            check_attention(g4, Setup(g4, spans, 1, hd, 64, fill=fill), 8, "f32", 0.1, 0, np.random.default_rng(6))
 
 
 def test_attention_nan_stays_in_its_sequence(g4):
@@ -480,10 +525,34 @@ def test_large_pool_offsets(g4):
     assert np.allclose(out.cpu().numpy()[0], want[0], rtol=2.0 ** -15, atol=0)
 
 
-def test_streams_and_graphs(g4):
+def test_large_pool_offsets_prompt(g4):
+    """A prompt on pages beyond 4 GB of the pool: the bits of one on a small pool's."""
+    hd, kv, page, rows = 512, 8, 1024, 200
+    size = g4.kv4_page_bytes(kv, hd, page)
+    rng = np.random.default_rng(4)
+    k, q = tensors(rng, rows, kv, hd, torch.float32), tensors(rng, rows, kv, hd, torch.float32)
+    off, start = dev([0, rows]), dev([900])
+    outs = []
+    for pages in (3, (1 << 32) // size + 3):
+        pool = torch.empty(pages * size, dtype=torch.uint8, device="cuda:0")
+        table = dev([[0, pages - 1]])
+        cache = g4.Kv4Cache(pool.data_ptr(), pages, page, kv, hd)
+        batch = g4.Kv4Batch(1, rows, off.data_ptr(), start.data_ptr(), table.data_ptr(), 2)
+        g4.kv4_write(cache, batch, 0, k.data_ptr(), k.stride(0), k.data_ptr(), k.stride(0))
+        out = torch.empty_like(q)
+        n = g4.kv4_attention_workspace(cache, batch, 0, kv)
+        ws = torch.empty(n, dtype=torch.uint8, device="cuda:0")
+        g4.kv4_attention(cache, batch, 0, kv, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), 0.1, 1,
+                         ws.data_ptr(), n)
+        outs.append(out)
+    assert torch.equal(*outs) and torch.isfinite(outs[0]).all() and outs[0][-1].any()
+
+
+@pytest.mark.parametrize("spans", [[(70, 2), (5, 1), (400, 1)], [(70, 200)]])
+def test_streams_and_graphs(g4, spans):
     """Write, attend and read on a side stream, then the same captured and replayed on new inputs."""
     rng = np.random.default_rng(11)
-    s = Setup(g4, [(70, 2), (5, 1), (400, 1)], 1, 256, 64)
+    s = Setup(g4, spans, 1, 256, 64)
     hist, _ = check_attention(g4, s, 8, "f32", 0.1, 0, rng)         # fills the cache
     k, v = tensors(rng, s.rows, 1, 256, torch.float32), tensors(rng, s.rows, 1, 256, torch.float32)
     q = tensors(rng, s.rows, 8, 256, torch.float32)
