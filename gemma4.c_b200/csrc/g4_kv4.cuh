@@ -120,6 +120,6 @@ cudaError_t g4_launch_kv4_attention(const Kv4View &c, int type, int q_heads, con
                                     cudaStream_t st);
 size_t g4_kv4_attention_ws(const Kv4View &c, int type, int q_heads);
 // g4_kv4_prompt.cu: the same for many query rows per sequence
-size_t kv4_prompt_ws(const Kv4View &c, int q_heads);
+size_t kv4_prompt_ws(const Kv4View &c, int type, int q_heads);
 cudaError_t kv4_launch_prompt(const Kv4View &c, int type, int q_heads, const void *q, long long q_stride, void *out,
                               long long out_stride, float scale, int window, void *ws, cudaStream_t st);

@@ -828,9 +828,9 @@ static bool many_rows(const Kv4View &c, int q_heads) {
     return (long long)c.rows * (q_heads / c.kv_heads) >= from * c.n;
 }
 
-size_t g4_kv4_attention_ws(const Kv4View &c, int, int q_heads) {
+size_t g4_kv4_attention_ws(const Kv4View &c, int type, int q_heads) {
     if (c.n == 0) return 16;
-    if (many_rows(c, q_heads)) return kv4_prompt_ws(c, q_heads);
+    if (many_rows(c, q_heads)) return kv4_prompt_ws(c, type, q_heads);
     return c.hd == 64 ? ws_bytes<64>() : c.hd == 128 ? ws_bytes<128>() : c.hd == 256 ? ws_bytes<256>() : ws_bytes<512>();
 }
 

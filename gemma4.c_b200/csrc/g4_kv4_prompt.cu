@@ -33,6 +33,12 @@ constexpr int kT = 64;             // keys of a tile: 4 records
 constexpr int kH = kT / 2;         // keys of a softmax thread
 constexpr int kSoftWarps = 8, kConvWarps = 8;
 constexpr int kThreads = (kSoftWarps + kConvWarps + 1) * 32;
+// Registers: five warps on one of an SM's four parts leave 96 a thread, on which the
+// softmax spilled in its loop (chunk of 512 tokens at 16384: 532 us). The conversion
+// gives it some of its own: 455 us.
+constexpr int kRegs = 96, kSoftRegs = 112, kConvRegs = 80;
+static_assert(kSoftWarps * kSoftRegs + kConvWarps * kConvRegs <= (kSoftWarps + kConvWarps) * kRegs,
+              "the block has what its warps take");
 constexpr int kSms = 148;
 constexpr int kJoinThreads = 256;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -51,6 +57,11 @@ struct Cfg {
     static constexpr int kQ = G * kM * 128;                  // one half of q: G tiles of 128 rows x 128 bytes
     static constexpr int kK = G * kT * 128;
     static constexpr int kV = kDc * 128;                     // V^T: rows are dimensions, 64 keys
+    // The tensor cores truncate as they add up, 8 steps a tile: an error that grows with
+    // the length of a run (fp32, 128 tiles: 2e-5 of the output, 4e-5 where values have one
+    // sign). So O is added to a sum in memory, in fp32, after every kRun tiles; 16-bit
+    // outputs round by more than that up to 256.
+    static constexpr int kRun = HILO ? 32 : 256;
     static constexpr int kX = kCl > 1 ? kM * kT * 4 : 0;     // the other CTA's half of S
     static constexpr int kSmem = kQ * (HILO ? 2 : 1) + kK + kV + kX;
 };
@@ -66,7 +77,7 @@ struct PromptP {
     long long q_stride, out_stride;
     float scale;
     int window;
-    float *parts, *stats;          // [slots][kv heads][splits][128][HD], [..][2][128]
+    float *parts, *stats;          // [slots][kv heads][splits][HD / 4][128][4], [..][2][128]
 };
 
 G4_DEV float ex2(float x) {
@@ -151,6 +162,12 @@ G4_DEV void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
         : "memory");
 }
 G4_DEV void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Four values added to memory without waiting for them
+G4_DEV void red_add4(float *p, float x, float y, float z, float w) {
+    asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(p), "f"(x), "f"(y), "f"(z), "f"(w)
+                 : "memory");
+}
 
 G4_DEV void load8(const void *p, int type, long long i, float (&x)[8]) {
     if (type == G4_TYPE_F32) Kv4Vec<float>::load((const float *)p + i, x);
@@ -406,7 +423,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
 #pragma unroll
                         for (int i = 0; i < kT / 16; i++)
                             mma_f16_ta(tmem + kColO, tmem + kColP + b * 64 + half * 32 + i * 8, umma_desc(vb, i * 32),
-                                       kIdO, j || half || i);
+                                       kIdO, j % C::kRun || half || i);
                     mma_commit(&odone[b]);
                 }
                 if (j + 2 < nt) {
@@ -425,6 +442,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
         }
         __syncwarp();
     } else if (warp >= kSoftWarps) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kConvRegs));
         // ---- conversion: this warp's record of each tile, its groups g0, g0 + 2, ... ----
         const int cw = warp - kSoftWarps, rec = cw & 3, g0 = cw >> 2;
         const bool busy = g0 < G;
@@ -610,6 +628,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
             if (j + 3 < nt) fetch_k(r2);
         }
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
         // ---- softmax: threads (r, half) take keys 32 half .. + 31 of row r ----
         const int quad = warp & 3, half = warp >> 2, r = quad * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
@@ -625,6 +644,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
         const uint32_t peer_free = CL > 1 ? rank_addr(smem_u32(&xfree[warp]), rank ^ 1) : 0;
         float m = -INFINITY, l = 0.0f;
         uint32_t nans = 0;                                      // groups with a NaN value that this row sees
+        // the row's sum of the runs before this one, in the range's place among the partial
+        // results (4 dimensions x rows, so that a warp's accesses are 512 bytes), for the reference m_acc
+        auto sums = [&]() { return p.parts + (long long)(blockIdx.x / CL) * (kM * HD) + rank * (kM * DC) + r * 4; };
+        float m_acc = -INFINITY;
+        auto factor = [&]() { return m_acc == m ? 1.0f : ex2(m_acc - m); };
         // this CTA's half of S of a tile to the other CTA: on its way while the tile before
         // it is worked on
         const int x0 = (half * (kH / 4)) * kM + r;
@@ -701,12 +725,40 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
             pair[b][half][r] = mx;
             bar_sync(1 + quad, 64);
             mx = fmaxf(mx, pair[b][half ^ 1][r]) * rs;
-            const bool grow = mx > m + kSlack;
+            const bool grow = mx > m + kSlack, turn = j > 0 && j % C::kRun == 0;
+            if (turn) {                                         // the run up to tile j - 1 is complete
+                wait(&odone[b ^ 1], (j - 1) >> 1);
+                tc_fence_after();
+                const float f = factor();
+                float *acc = sums();
+                // Nothing but this thread touches its sums, so additions in memory have one
+                // order. The reference rarely moves once a few tiles are done.
+                const bool same = __all_sync(0xffffffffu, f == 1.0f), first = j == C::kRun;
+#pragma unroll 1
+                for (int c = half * (DC / 2); c < (half + 1) * (DC / 2); c += 32) {
+                    int v[32];
+                    tmem_ld32(lanes + kColO + c, v);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int x = 0; x < 32; x += 4) {
+                        float4 *to = reinterpret_cast<float4 *>(acc + (c + x) * kM);
+                        float4 y = make_float4(__int_as_float(v[x]), __int_as_float(v[x + 1]), __int_as_float(v[x + 2]),
+                                               __int_as_float(v[x + 3]));
+                        if (first) __stcg(to, y);
+                        else if (same) red_add4(&to->x, y.x, y.y, y.z, y.w);
+                        else {
+                            const float4 z = __ldcg(to);
+                            __stcg(to, make_float4(fmaf(z.x, f, y.x), fmaf(z.y, f, y.y), fmaf(z.z, f, y.z), fmaf(z.w, f, y.w)));
+                        }
+                    }
+                }
+                m_acc = m;
+            }
             if (__any_sync(0xffffffffu, grow)) {                // the same in both warps of the rows
                 const float mn = grow ? mx + kHead : m, al = mn == m ? 1.0f : ex2(m - mn);
                 m = mn;
                 l *= al;
-                if (j > 0) {
+                if (j > 0 && !turn) {                           // (after a turn the next P V starts O anew)
                     wait(&odone[b ^ 1], (j - 1) >> 1);          // O is complete up to tile j - 1
                     tc_fence_after();
                     for (int c = half * (DC / 2); c < (half + 1) * (DC / 2); c += 32) {
@@ -750,7 +802,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
         l += pair[0][half ^ 1][r];
         nans |= __float_as_uint(pair[1][half][r]) | __float_as_uint(pair[1][half ^ 1][r]);
         const bool part = p.splits > 1;
-        const long long item = (long long)(slot * p.c.kv_heads + h) * p.splits + split;
+        const long long item = blockIdx.x / CL;
+        float *acc = sums();
+        const float f = factor();
         const float fac = pow2(min(17 - va, 127)) * (part ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l);
         if (part && rank == 0 && half == 0) {
             p.stats[item * (2 * kM) + r] = m;
@@ -766,13 +820,26 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
 #pragma unroll
                 for (int x = 0; x < 32; x++) v[x] = 0;
             }
+            if (nt > C::kRun) {
+#pragma unroll
+                for (int x = 0; x < 32; x += 4) {
+                    const float4 y = __ldcg(reinterpret_cast<const float4 *>(acc + (c + x) * kM));
+                    v[x] = __float_as_int(fmaf(y.x, f, __int_as_float(v[x])));
+                    v[x + 1] = __float_as_int(fmaf(y.y, f, __int_as_float(v[x + 1])));
+                    v[x + 2] = __float_as_int(fmaf(y.z, f, __int_as_float(v[x + 2])));
+                    v[x + 3] = __float_as_int(fmaf(y.w, f, __int_as_float(v[x + 3])));
+                }
+            }
             const bool bad = nans >> (c / kKv4Group) & 1;
 #pragma unroll
             for (int x = 0; x < 32; x += 8) {
                 float y[8];
 #pragma unroll
                 for (int i = 0; i < 8; i++) y[i] = bad ? NAN : __int_as_float(v[x + i]) * fac;
-                if (part) Kv4Vec<float>::store(p.parts + (item * kM + r) * HD + rank * DC + c + x, y);
+                if (part) {
+                    *reinterpret_cast<float4 *>(acc + (c + x) * kM) = make_float4(y[0], y[1], y[2], y[3]);
+                    *reinterpret_cast<float4 *>(acc + (c + x + 4) * kM) = make_float4(y[4], y[5], y[6], y[7]);
+                }
                 else if (r < valid)
                     store8(p.out, p.type, q_row(r) * p.out_stride + head_of(r) + rank * DC + c + x, y);
             }
@@ -792,7 +859,7 @@ template <int HD>
 __global__ void __launch_bounds__(kJoinThreads) k_kv4_prompt_join(const __grid_constant__ PromptP p) {
     __shared__ float f[32][8], inv[8];
     const int tid = threadIdx.x, r0 = blockIdx.y * 8;
-    const int slot = blockIdx.x / p.c.kv_heads, h = blockIdx.x % p.c.kv_heads;
+    const int slot = p.slots - 1 - blockIdx.x / p.c.kv_heads, h = blockIdx.x % p.c.kv_heads;      // as the kernel before
     griddep_wait();
     Item it;
     if (!find_item(p, slot, it)) return;
@@ -813,12 +880,14 @@ __global__ void __launch_bounds__(kJoinThreads) k_kv4_prompt_join(const __grid_c
     }
     __syncthreads();
     for (int i = tid; i < HD; i += kJoinThreads) {              // 8 rows of HD / 8 pieces
-        const int r = i / (HD / 8), d = i % (HD / 8) * 8;
+        const int r = i % 8, d = i / 8 * 8;
+        const float *from = p.parts + item * (kM * HD) + (d * kM + (r0 + r) * 4);
         float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
         for (int s = 0; s < p.splits; s++) {
-            float y[8];
-            Kv4Vec<float>::load(p.parts + ((item + s) * kM + r0 + r) * HD + d, y);
+            __align__(16) float y[8];
+            *reinterpret_cast<float4 *>(y) = *reinterpret_cast<const float4 *>(from + s * (kM * HD));
+            *reinterpret_cast<float4 *>(y + 4) = *reinterpret_cast<const float4 *>(from + s * (kM * HD) + 4 * kM);
 #pragma unroll
             for (int j = 0; j < 8; j++) x[j] = fmaf(f[s][r], y[j], x[j]);
         }
@@ -871,6 +940,11 @@ cudaError_t launch_prompt(const PromptP &p, cudaStream_t st) {
     using C = Cfg<HD, HILO>;
     cudaError_t e = g4_smem_optin((const void *)k_kv4_prompt<HD, HILO>, C::kSmem);
     if (e != cudaSuccess) return e;
+    static const bool fits = [] {                               // a build with fewer registers would wait for more
+        cudaFuncAttributes a;
+        return cudaFuncGetAttributes(&a, (const void *)k_kv4_prompt<HD, HILO>) == cudaSuccess && a.numRegs >= kRegs;
+    }();
+    if (!fits) return cudaErrorLaunchOutOfResources;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)p.slots * p.c.kv_heads * p.splits * C::kCl);
     cfg.blockDim = dim3(kThreads);
@@ -897,10 +971,12 @@ cudaError_t launch_hd(const PromptP &p, cudaStream_t st) {
 
 }  // namespace
 
-size_t kv4_prompt_ws(const Kv4View &c, int q_heads) {
+size_t kv4_prompt_ws(const Kv4View &c, int type, int q_heads) {
     int tokens, slots, splits;
     plan(c, q_heads / c.kv_heads, 0, &tokens, &slots, &splits);
-    return splits == 1 ? 16 : (size_t)slots * c.kv_heads * splits * kM * (c.hd + 2) * sizeof(float);
+    const int run = type == G4_TYPE_F32 ? Cfg<64, true>::kRun : Cfg<64, false>::kRun;
+    const bool runs = ((long long)c.table_stride << c.page_shift) > run * kT;      // of tiles, to be summed up
+    return splits == 1 && !runs ? 16 : (size_t)slots * c.kv_heads * splits * kM * (c.hd + 2) * sizeof(float);
 }
 
 cudaError_t kv4_launch_prompt(const Kv4View &c, int type, int q_heads, const void *q, long long q_stride, void *out,
