@@ -304,16 +304,24 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
     };
     auto head_of = [&](int r) { return (long long)(h * p.group + (unsigned)r % p.group) * HD; };
 
-    // ---- prologue: query operands (all but the MMA warp), largest scales (conversion warps) ----
+    // ---- prologue, all but the MMA warp: query operands, largest scales ----
+    const int recs = nt * (kT / kKv4Rec);
+    auto scan_addr = [&](int r0) -> unsigned long long {        // of this warp's next 32 records, one per lane
+        const int mine = r0 + warp + lane * (kSoftWarps + kConvWarps);
+        return mine < recs ? (unsigned long long)kv4_record(p.c, it.seq, (long long)t0 * kT + mine * kKv4Rec, h) : 0;
+    };
+    unsigned long long addr = 0;
+    if (warp < kSoftWarps + kConvWarps) addr = scan_addr(0);
     if (warp < kSoftWarps + kConvWarps) {
         constexpr int LR = DC / 8 < 32 ? DC / 8 : 32;           // lanes of a row
         constexpr int RP = 32 / LR, RW = kM / (kSoftWarps + kConvWarps), NP = RW / RP;   // rows of a pass, of a warp
+        constexpr int NU = NP < 4 ? NP : 4;                     // passes in flight
         const int lr = lane / LR, ch = lane % LR;
 #pragma unroll 1
-        for (int p0 = 0; p0 < NP; p0 += 2) {
-            float x[2][8];
+        for (int p0 = 0; p0 < NP; p0 += NU) {
+            float x[NU][8];
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
+            for (int u = 0; u < NU; u++) {
                 const int r = warp * RW + (p0 + u) * RP + lr;
 #pragma unroll
                 for (int i = 0; i < 8; i++) x[u][i] = 0.0f;
@@ -321,7 +329,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
                     load8(p.q, p.type, q_row(r) * p.q_stride + head_of(r) + rank * DC + ch * 8, x[u]);
             }
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
+            for (int u = 0; u < NU; u++) {
                 if (p0 + u >= NP) break;
                 const int r = warp * RW + (p0 + u) * RP + lr;
                 float mx = 0.0f;
@@ -350,37 +358,41 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
         }
         fence_async();
     }
-    if (warp >= kSoftWarps && warp < kSoftWarps + kConvWarps) {
+    if (warp < kSoftWarps + kConvWarps) {
+        // The largest scales: a warp takes every 16th record, 8 at a time in flight, K scales
+        // of a token per lane in its lower half, G V scales per lane in the upper one.
+        constexpr int kScan = kSoftWarps + kConvWarps, kFlight = 8;
         uint32_t km = 0, vm = 0;
-        const int cw = warp - kSoftWarps, recs = nt * (kT / kKv4Rec);
-        for (int r0 = 0; r0 < recs; r0 += 32 * kConvWarps) {
-            // addresses of this warp's next 32 records, one per lane
-            const int mine = r0 + cw + lane * kConvWarps;
-            unsigned long long addr = 0;
-            if (mine < recs) addr = (unsigned long long)kv4_record(p.c, it.seq, (long long)t0 * kT + mine * 16, h);
-#pragma unroll 4
-            for (int k = 0; k < 32; k++) {
-                const int rec = r0 + cw + k * kConvWarps;
-                if (rec >= recs) break;
-                const uint8_t *src = (const uint8_t *)__shfl_sync(0xffffffffu, addr, k);
-                if (!src) continue;
-                // lanes 0-15: the K scales of a token, 16-31: G of the V scales
-                const bool is_v = lane >= 16;
-                const int i = lane & 15, key = t0 * kT + rec * 16;
-                const uint8_t *from = src + 16 * HD + (is_v ? 32 * HG + rank * (32 * G) + i * (2 * G)
-                                                            : i * (2 * HG) + rank * (2 * G));
-                uint32_t w[2] = {0, 0};
-                if constexpr (G == 4) {
-                    const uint2 x = *reinterpret_cast<const uint2 *>(from);
-                    w[0] = x.x;
-                    w[1] = x.y;
-                } else if constexpr (G == 2) w[0] = *reinterpret_cast<const uint32_t *>(from);
-                else w[0] = *reinterpret_cast<const uint16_t *>(from);
+        const bool is_v = lane >= 16;
+        const int i16 = lane & 15, at_lane = 16 * HD + (is_v ? 32 * HG + rank * (32 * G) + i16 * (2 * G)
+                                                              : i16 * (2 * HG) + rank * (2 * G));
+        for (int r0 = 0; r0 < recs; r0 += 32 * kScan) {
+            if (r0) addr = scan_addr(r0);
+            const int left = (recs - r0 - warp + kScan - 1) / kScan;
+            for (int k0 = 0; k0 < min(left, 32); k0 += kFlight) {
+                uint32_t w[kFlight][2];
 #pragma unroll
-                for (int x = 0; x < G; x++) {
-                    const uint32_t a = w[x / 2] >> (16 * (x & 1)) & 0xffffu;
-                    const int at = i * G + x, tok = is_v ? 2 * (at >> 2 & 3) + (at & 1) + 8 * (at >> 1 & 1) : i;
-                    if (key + tok >= it.see0 && key + tok <= it.see1 && a < 0x7f80u) km = max(km, a);
+                for (int u = 0; u < kFlight; u++) {
+                    const uint8_t *src = (const uint8_t *)__shfl_sync(0xffffffffu, addr, k0 + u);
+                    w[u][0] = w[u][1] = 0;
+                    if (!src) continue;
+                    if constexpr (G == 4) {
+                        const uint2 x = *reinterpret_cast<const uint2 *>(src + at_lane);
+                        w[u][0] = x.x;
+                        w[u][1] = x.y;
+                    } else if constexpr (G == 2) w[u][0] = *reinterpret_cast<const uint32_t *>(src + at_lane);
+                    else w[u][0] = *reinterpret_cast<const uint16_t *>(src + at_lane);
+                }
+#pragma unroll
+                for (int u = 0; u < kFlight; u++) {
+                    const int key = t0 * kT + (r0 + warp + (k0 + u) * kScan) * kKv4Rec;
+                    const bool inside = key >= it.see0 && key + kKv4Rec - 1 <= it.see1;
+#pragma unroll
+                    for (int x = 0; x < G; x++) {
+                        const uint32_t a = w[u][x / 2] >> (16 * (x & 1)) & 0xffffu;
+                        const int at = i16 * G + x, tok = is_v ? 2 * (at >> 2 & 3) + (at & 1) + 8 * (at >> 1 & 1) : i16;
+                        if (a < 0x7f80u && (inside || (key + tok >= it.see0 && key + tok <= it.see1))) km = max(km, a);
+                    }
                 }
             }
         }
