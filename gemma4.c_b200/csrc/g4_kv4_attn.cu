@@ -54,6 +54,7 @@ struct Cfg {
     static constexpr int kStages = HD >= 256 ? 3 : HD == 128 ? 4 : 6;
     static constexpr int kOcc = HD == 512 ? 1 : 2;
     static constexpr int kCtas = kSms * kOcc;
+    static constexpr int kWhole = HD >= 256 ? 40 : 64;          // records of an item that is not cut
     static constexpr int kRing = kStreams * kStages * kRec;
     static constexpr int kQ = G * 1024;                         // operands of the query tile (one half)
     static constexpr int kPad = HD + 2;                        // row of a warp's output when the warps meet
@@ -70,6 +71,7 @@ struct AttnP {
     long long q_stride, out_stride;
     float scale;
     int window;
+    int whole;                    // items are not cut: there is nothing to join
     float *slots;                 // partial outputs [2 per CTA][8][HD]
     float *stats;                 // their maxima and sums [2 per CTA][2][8]
 };
@@ -312,7 +314,7 @@ G4_DEV void next_item(const AttnP &p, Walk &w, Item &out) {
     const Seq s = w.seqs[b - w.cached];
     // units [u0, u1) of the item, of which the first kItemCost are no records: who
     // holds only such leaves the item to the next CTA
-    const int u0 = w.unit, u1 = (int)min((long long)s.recs + kItemCost, u0 + w.left);
+    const int size = s.recs + kItemCost, u0 = w.unit, u1 = p.whole ? size : (int)min((long long)size, u0 + w.left);
     const int r0 = max(u0 - kItemCost, 0), r1 = u1 - kItemCost;
     w.left -= u1 - u0;
     w.b = b;
@@ -378,7 +380,13 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kOcc) k_kv4_attn(const __gr
             walk.left = min(total - w0, share);
             walk.b = scan.seq;
             walk.cached = -kSeqs;
-            divide(scan.off, seq_of(p, scan.seq).recs + kItemCost, walk.item, walk.unit);
+            const int size = seq_of(p, scan.seq).recs + kItemCost;
+            divide(scan.off, size, walk.item, walk.unit);
+            if (p.whole && walk.unit) {                                 // the CTA has the items that start in its share
+                walk.left -= size - walk.unit;
+                walk.item++;
+                walk.unit = 0;
+            }
         }
         __syncwarp();
         next_item(p, walk, items[0]);
@@ -798,12 +806,22 @@ cudaError_t launch_stream(const AttnP &p, cudaStream_t st) {
     cudaError_t e = g4_smem_optin((const void *)k_kv4_attn<HD, HILO>, smem);
     if (e != cudaSuccess) return e;
     e = g4_launch(k_kv4_attn<HD, HILO>, dim3(C::kCtas), dim3(kThreads), (size_t)smem, st, true, p);
-    if (e != cudaSuccess) return e;
+    if (e != cudaSuccess || p.whole) return e;
     return g4_launch(k_kv4_attn_join<HD>, dim3(C::kCtas - 1), dim3(kJoinThreads), 0, st, true, p);
 }
 
 template <int HD>
 cudaError_t launch_hd(AttnP &p, cudaStream_t st) {
+    // Items of few records, not more of them than CTAs: a CTA has an item for itself, and the
+    // second kernel is saved. One token of 8 heads and a window of 512 tokens (33 records), us
+    // cut and whole: 64 dimensions, 1 / 64 / 128 sequences 9.7 / 7.7, 12.5 / 9.4, 16.4 / 9.8; 256
+    // dimensions 13.6 / 13.0, 19.0 / 18.1, 23.2 / 19.2; 512 dimensions 17.5 / 18.1, 19.9 / 19.1,
+    // 28.1 / 28.2. At 1000 tokens (63 records): 64 dimensions 9.7 / 9.7, 16.1 / 12.4, 18.4 / 12.7;
+    // 256 dimensions 13.6 / 17.8, 23.1 / 26.3, 30.1 / 27.9.
+    const long long cap = (long long)p.c.table_stride << p.c.page_shift,
+                    seen = p.window && (long long)p.window + kRows < cap ? (long long)p.window + kRows : cap,
+                    tiles = (long long)p.c.rows * p.group / kRows + p.c.n;
+    p.whole = seen <= Cfg<HD>::kWhole * kKv4Rec && tiles * p.c.kv_heads <= Cfg<HD>::kCtas;
     p.stats = p.slots + (size_t)2 * Cfg<HD>::kCtas * Cfg<HD>::kSlot;
     return p.type == G4_TYPE_F32 ? launch_stream<HD, true>(p, st) : launch_stream<HD, false>(p, st);
 }

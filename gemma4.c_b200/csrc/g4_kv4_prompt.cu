@@ -320,14 +320,22 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
 #pragma unroll 1
         for (int p0 = 0; p0 < NP; p0 += NU) {
             float x[NU][8];
+            uint4 raw[NU];                                      // of 16-bit types, so that all loads are on their way at once
 #pragma unroll
             for (int u = 0; u < NU; u++) {
                 const int r = warp * RW + (p0 + u) * RP + lr;
+                const bool have = p0 + u < NP && r < valid;
+                const long long at = have ? q_row(r) * p.q_stride + head_of(r) + rank * DC + ch * 8 : 0;
 #pragma unroll
                 for (int i = 0; i < 8; i++) x[u][i] = 0.0f;
-                if (p0 + u < NP && r < valid)
-                    load8(p.q, p.type, q_row(r) * p.q_stride + head_of(r) + rank * DC + ch * 8, x[u]);
+                raw[u] = make_uint4(0, 0, 0, 0);
+                if (HILO) {
+                    if (have) Kv4Vec<float>::load((const float *)p.q + at, x[u]);
+                } else if (have) raw[u] = *reinterpret_cast<const uint4 *>((const uint16_t *)p.q + at);
             }
+#pragma unroll
+            for (int u = 0; u < NU && !HILO; u++)
+                load8(&raw[u], p.type, 0, x[u]);
 #pragma unroll
             for (int u = 0; u < NU; u++) {
                 if (p0 + u >= NP) break;
@@ -916,14 +924,14 @@ __global__ void __launch_bounds__(kJoinThreads) k_kv4_prompt_join(const __grid_c
 
 // Key ranges of a row tile that sees `tiles` key tiles, by the time of the rounds that
 // the row tiles then take: a key tile costs 1, a range (its queries, scales and output)
-// about 5. At most 32, and four rounds: more would not fill the GPU better, and the
+// about 3. At most 32, and four rounds: more would not fill the GPU better, and the
 // partial outputs would grow.
 int ranges(const Kv4View &c, long long items, long long tiles) {
     const long long room = kSms / (c.hd > 256 ? 2 : 1);
     double best = 0.0;
     int n = 1;
     for (int s = 1; s <= 32 && s <= tiles && (s == 1 || items * s <= 4 * room); s++) {
-        const double cost = (double)((items * s + room - 1) / room) * ((double)tiles / s + 5.0);
+        const double cost = (double)((items * s + room - 1) / room) * ((double)tiles / s + 3.0);
         if (s == 1 || cost < 0.97 * best) {
             best = cost;
             n = s;

@@ -276,6 +276,18 @@ def test_attention_window(g4, window, hd, heads):
     check_attention(g4, s, heads, "f32", 0.2, window, rng, pad=128)
 
 
+@pytest.mark.parametrize("hd,heads,kv", [(64, 8, 1), (128, 6, 2), (256, 8, 1), (512, 8, 1)])
+@pytest.mark.parametrize("n", [1, 40, 140])
+def test_attention_items_of_few_records(g4, n, hd, heads, kv):
+    """Windows and tables of few records, where a CTA has an item for itself, beside ones
+    that are just too long or too many for that; empty sequences and rows between them."""
+    rng = np.random.default_rng(n)
+    spans = [(int(p), int(rng.integers(0, 4))) for p in rng.integers(0, 900, n)]
+    for window in (17, 600, 640, 1016, 1017):
+        check_attention(g4, Setup(g4, spans, kv, hd, 64), heads, "f32", 0.1, window, rng)
+    check_attention(g4, Setup(g4, [(p % 200, q) for p, q in spans], kv, hd, 16), heads, "bf16", 0.1, 0, rng)
+
+
 @pytest.mark.parametrize("hd,heads,kv,name", [(512, 8, 1, "f32"), (256, 8, 1, "f32"), (128, 32, 8, "bf16"),
                                               (64, 8, 1, "f16")])
 def test_attention_long(g4, hd, heads, kv, name):
