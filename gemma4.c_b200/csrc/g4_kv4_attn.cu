@@ -31,6 +31,15 @@
 // head) and cut into one even run per CTA, so ragged batches and one long
 // sequence fill the GPU alike; a sequence cut between CTAs leaves partial
 // results that a second kernel joins in order.
+//
+// Measured (GPU time, both kernels): 64 sequences of 128 to 8704 tokens, one kv head of
+// 512 dimensions, 8 fp32 query heads each 36 us (79 MB of records, 12.1 us at HBM's
+// rate); one sequence of 131072 tokens 33 us (10.9); 32 sequences up to 16384, 8 kv heads
+// of 128 dimensions, 32 bf16 heads 39 us (12.1); a window of 512 tokens 13 us. An SM
+// takes about 570 clocks for a record of 512 dimensions where its share of HBM delivers
+// one in 378: 128 MMAs and the ANDs, shifts and adds of the codes share the issue. Not better:
+// two warps a record, Q K of the next record beside P V, separate accumulators for the
+// high and low halves.
 #include <cuda_runtime.h>
 
 #include "g4_kv4.cuh"
@@ -834,15 +843,16 @@ size_t ws_bytes() {
 }  // namespace
 
 // Many query rows per sequence and kv head go to the tcgen05 tiles of 128 rows, few to
-// this file's tiles of 8, whose time grows with the rows while the other's starts at 30
-// (256 dimensions) to 50 us (512) for a context of 4000. Measured on either side, us here
-// and there: 16 sequences, 512 dimensions, 16 tokens x 8 heads on average 126 / 145, 33
-// tokens 234 / 209; 128 dimensions, 8 kv heads, 33 tokens x 4 heads 249 / 275, 65 tokens
-// 475 / 313; one sequence of 512 dimensions and one kv head, 64 tokens x 8 heads 47 / 54,
-// 128 tokens 80 / 60, of 256 dimensions 35 / 35 and 50 / 41. Fewer than four sequences and
-// heads of many dimensions leave the large tiles less to share out, hence their own bound.
+// this file's tiles of 8, whose time grows with the rows while the other's starts at 33
+// (256 dimensions) to 43 us (512) for a context of 4000. Measured on either side, us here
+// and there: 16 sequences, 512 dimensions, 8 tokens x 8 heads on average 71 / 120, 16 tokens
+// 127 / 124, 33 tokens 236 / 176; 256 dimensions, 16 tokens 74 / 69; 128 dimensions, 8 kv heads
+// of 4, 16 tokens 134 / 169, 33 tokens 250 / 205. Fewer than four sequences and heads of many
+// dimensions leave the large tiles less to share out: one sequence and kv head of 512
+// dimensions, 64 tokens x 8 heads 47 / 50, 128 tokens 80 / 53; of 256 dimensions 35 / 37 and
+// 51 / 36. Hence their own bound.
 static bool many_rows(const Kv4View &c, int q_heads) {
-    const long long from = c.hd >= 256 && (long long)c.n * c.kv_heads < 4 ? 512 : 160;
+    const long long from = c.hd >= 256 && (long long)c.n * c.kv_heads < 4 ? 576 : 112;
     return (long long)c.rows * (q_heads / c.kv_heads) >= from * c.n;
 }
 

@@ -21,6 +21,16 @@
 // 8-15 conversion (each a record of the tile and some of its groups, the next tile's
 // codes in flight in registers), 16 the MMAs. S and P are double-buffered: while the softmax works on tile
 // j, the MMAs of P_{j-1} V and S_{j+1} run and K of tile j + 2 and V of tile j are converted.
+//
+// Measured: 512 tokens of 8 fp32 heads of 512 dimensions behind 15872 428 us (316 TFLOP/s
+// of the operator's, twice that on the tensor cores, which work on two terms of q and of
+// p); 2048 tokens of 256 dimensions behind 6144 289 us (417); 2048 tokens of 32 bf16 heads
+// of 128 dimensions, 8 kv heads, 108 us (318). A tile takes 3.2 us at 512 dimensions, where
+// the MMAs need 1.4 and sending the halves of S (32 KB each way, st.async; plain remote
+// stores with one arrival a warp 522 us, sending before the maximum 463 us) bounds it; 2.1 us
+// at 256, where MMAs of 64 columns (48 clocks against 32 for their share) bound it.
+#include <atomic>
+
 #include <cuda_runtime.h>
 
 #include "g4_kv4.cuh"
@@ -923,15 +933,16 @@ __global__ void __launch_bounds__(kJoinThreads) k_kv4_prompt_join(const __grid_c
 }
 
 // Key ranges of a row tile that sees `tiles` key tiles, by the time of the rounds that
-// the row tiles then take: a key tile costs 1, a range (its queries, scales and output)
-// about 3. At most 32, and four rounds: more would not fill the GPU better, and the
+// the row tiles then take: a key tile costs 1, a range (its queries and scales) about 3,
+// its partial result in memory hd / 20000. At most 32, and four rounds: more would not fill the GPU better, and the
 // partial outputs would grow.
 int ranges(const Kv4View &c, long long items, long long tiles) {
     const long long room = kSms / (c.hd > 256 ? 2 : 1);
     double best = 0.0;
     int n = 1;
     for (int s = 1; s <= 32 && s <= tiles && (s == 1 || items * s <= 4 * room); s++) {
-        const double cost = (double)((items * s + room - 1) / room) * ((double)tiles / s + 3.0);
+        const double cost = (double)((items * s + room - 1) / room) * ((double)tiles / s + 3.0) +
+                            (s > 1 ? (double)(items * s) * c.hd / 20000.0 : 0.0);
         if (s == 1 || cost < 0.97 * best) {
             best = cost;
             n = s;
@@ -960,11 +971,14 @@ cudaError_t launch_prompt(const PromptP &p, cudaStream_t st) {
     using C = Cfg<HD, HILO>;
     cudaError_t e = g4_smem_optin((const void *)k_kv4_prompt<HD, HILO>, C::kSmem);
     if (e != cudaSuccess) return e;
-    static const bool fits = [] {                               // a build with fewer registers would wait for more
+    static std::atomic<bool> fits{false};                       // a build with fewer registers would wait for more
+    if (!fits) {
         cudaFuncAttributes a;
-        return cudaFuncGetAttributes(&a, (const void *)k_kv4_prompt<HD, HILO>) == cudaSuccess && a.numRegs >= kRegs;
-    }();
-    if (!fits) return cudaErrorLaunchOutOfResources;
+        e = cudaFuncGetAttributes(&a, (const void *)k_kv4_prompt<HD, HILO>);
+        if (e != cudaSuccess) return e;
+        if (a.numRegs < kRegs) return cudaErrorLaunchOutOfResources;
+        fits = true;
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)p.slots * p.c.kv_heads * p.splits * C::kCl);
     cfg.blockDim = dim3(kThreads);
