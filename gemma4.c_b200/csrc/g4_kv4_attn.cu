@@ -422,6 +422,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kOcc) k_kv4_attn(const __gr
     };
 
     unsigned long long addr = 0;
+    bool lost = false;                        // a copy never came: this warp copies no more, its outputs are NaN
     float qx[QN][8];
     if (!items[0].none) {
         addr = lookup(items[0], 0);
@@ -431,7 +432,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kOcc) k_kv4_attn(const __gr
     for (int cur = 0; !items[cur].none; cur ^= 1) {
         const Item &it = items[cur];
         const int ra = it.ra, all0 = it.all0, all1 = it.all1;
-        const int nmine = max(0, (it.rb - ra - stream + kStreams - 1) / kStreams);    // records of this stream
+        const int nmine = lost ? 0 : max(0, (it.rb - ra - stream + kStreams - 1) / kStreams);    // records of this stream
         uint32_t there = 0;                 // stages that hold a record (not of a missing page)
         auto issue = [&](int k) {
             if (k >= nmine) return;
@@ -515,7 +516,6 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kOcc) k_kv4_attn(const __gr
         float m = -INFINITY, l = 0.0f;
         const float rs = row_scale[g];
 
-        bool lost = false;                                    // a copy that never came
         uint32_t ph0 = 0, ph1 = 0, pl0 = 0, pl1 = 0;          // p of a record as high and low bf16
         uint32_t see01 = 0, see23 = 0;                        // which of its keys row g sees, as masks of the scales
 
@@ -572,7 +572,12 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kOcc) k_kv4_attn(const __gr
             const uint8_t *rec = my_ring + st * REC;
             const bool here = there >> st & 1;                // a missing page has no keys
             if (here) {
-                if (!mbar_wait(&full[stream][st], phase >> st & 1, nullptr, 0)) lost = true;
+                if (!__all_sync(0xffffffffu, mbar_wait(&full[stream][st], phase >> st & 1, nullptr, 0))) {
+                    lost = true;                              // the others in flight are waited for, with the same limit
+                    for (int i = 0; i < ST; i++)
+                        if (there >> i & 1 && i != st) mbar_wait(&full[stream][i], phase >> i & 1, nullptr, 0);
+                    break;
+                }
                 phase ^= 1u << st;
                 float sc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                 uint32_t k0s[(G + 1) / 2], k1s[(G + 1) / 2];  // scales of keys g and g + 8

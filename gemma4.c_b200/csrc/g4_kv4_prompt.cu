@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
     constexpr int G = C::G, HG = HD / kKv4Group, DC = C::kDc, CL = C::kCl;
     constexpr int NB = G > 1 ? G / 2 : 1;                       // groups of a conversion warp
     extern __shared__ __align__(1024) uint8_t base[];          // tiles with the 128-byte swizzle
-    __shared__ uint64_t kfull, vfull, sfull[2], pfull[2], odone[2];
+    __shared__ uint64_t kfull, vfull, ended, sfull[2], pfull[2], odone[2];
     __shared__ uint64_t xfull[kSoftWarps], xfree[kSoftWarps];   // a softmax warp and its like in the other CTA
     __shared__ uint32_t tmem_slot;
     __shared__ float pair[2][2][kM];                            // between the two threads of a row
@@ -279,6 +279,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
     if (tid == 0) {
         mbar_init(&kfull, kConvWarps);
         mbar_init(&vfull, kConvWarps);
+        mbar_init(&ended, 1);
         for (int i = 0; i < 2; i++) {
             mbar_init(&sfull[i], 1);
             mbar_init(&odone[i], 1);
@@ -468,6 +469,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
                                     umma_desc(kb + (i >> 2) * (kT * 128), (i & 3) * 32), kIdS, half || i);
                     mma_commit(&sfull[j & 1]);
                 }
+            }
+            if (lost) {                                         // no MMA is left when TMEM is freed
+                mma_commit(&ended);
+                mbar_wait(&ended, 0, nullptr, 0);
             }
         }
         __syncwarp();
