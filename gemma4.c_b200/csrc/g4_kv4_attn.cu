@@ -24,7 +24,9 @@
 //                keys and an offset there would add up the truncations of the tensor
 //                core. p is 2^80 times too large to keep sums away from 2^-126: values
 //                up to 2^38 times a code are safe. p vs is split into high and low
-//                bf16 (16 bits) by packed FMAs on p's own halves.
+//                bf16: for fp32 outputs from the fp32 product (2^-18 of it is lost; with
+//                the next form outputs were 6.8e-6 off instead of 4.1e-6, a 64-sequence
+//                step took 2 % less), for others by packed FMAs on p's own halves (16 bits).
 // Every warp streams its own records of 16 keys through a ring in shared memory
 // and keeps its own running maximum, sum and output; the warps meet once per
 // sequence and head. Work is counted in records over all (sequence, row tile, kv
@@ -34,7 +36,7 @@
 //
 // Measured (GPU time, both kernels): 64 sequences of 128 to 8704 tokens, one kv head of
 // 512 dimensions, 8 fp32 query heads each 36 us (79 MB of records, 12.1 us at HBM's
-// rate); one sequence of 131072 tokens 33 us (10.9); 32 sequences up to 16384, 8 kv heads
+// rate); one sequence of 131072 tokens 34 us (10.9); 32 sequences up to 16384, 8 kv heads
 // of 128 dimensions, 32 bf16 heads 39 us (12.1); a window of 512 tokens 13 us. An SM
 // takes about 570 clocks for a record of 512 dimensions where its share of HBM delivers
 // one in 378: 128 MMAs and the ANDs, shifts and adds of the codes share the issue. Not better:
@@ -185,6 +187,13 @@ G4_DEV void load_scales(const void *p, uint32_t (&w)[(N + 1) / 2]) {
     else w[0] = *reinterpret_cast<const uint16_t *>(p);
 }
 G4_DEV float half_of(uint32_t w, int i) { return __uint_as_float(i ? w & 0xffff0000u : w << 16); }
+
+// p times two bf16 scales as high and low bf16: 2^-18 of the product is lost
+G4_DEV void split(uint64_t p, uint32_t vs, uint32_t &h, uint32_t &l) {
+    const float2 x = upk(mul2(p, pk(half_of(vs, 0), half_of(vs, 1))));
+    h = pack_b(x.x, x.y);
+    l = pack_b(x.x - half_of(h, 0), x.y - half_of(h, 1));
+}
 
 constexpr int kItemCost = 16;
 constexpr int kSeqs = 32;         // sequences described in shared memory at a time
@@ -517,6 +526,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kOcc) k_kv4_attn(const __gr
         const float rs = row_scale[g];
 
         uint32_t ph0 = 0, ph1 = 0, pl0 = 0, pl1 = 0;          // p of a record as high and low bf16
+        uint64_t p01 = 0, p23 = 0;                            // with fp32 outputs: as it is
         uint32_t see01 = 0, see23 = 0;                        // which of its keys row g sees, as masks of the scales
 
         // scores of one group: lane holds keys g, g + 8 x rows 2t, 2t + 1
@@ -553,10 +563,16 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kOcc) k_kv4_attn(const __gr
             uint2 vs = reinterpret_cast<const uint2 *>(rec + 16 * HD + 32 * G)[gr * 4 + t];
             vs.x &= see01;                                    // the scale of a token that is not seen may be anything
             vs.y &= see23;
-            // p vs = h + l: h the rounded product of p's high half, l what it lost and the low half's product
-            const uint32_t h0 = mul_b(ph0, vs.x), h1 = mul_b(ph1, vs.y);
-            const uint32_t l0 = fma_b(pl0, vs.x, fma_b(ph0, vs.x, h0 ^ 0x80008000u));
-            const uint32_t l1 = fma_b(pl1, vs.y, fma_b(ph1, vs.y, h1 ^ 0x80008000u));
+            uint32_t h0, h1, l0, l1;                          // p vs = h + l
+            if constexpr (HILO) {
+                split(p01, vs.x, h0, l0);
+                split(p23, vs.y, h1, l1);
+            } else {
+                // h the rounded product of p's high half, l what it lost and the low half's product
+                h0 = mul_b(ph0, vs.x), h1 = mul_b(ph1, vs.y);
+                l0 = fma_b(pl0, vs.x, fma_b(ph0, vs.x, h0 ^ 0x80008000u));
+                l1 = fma_b(pl1, vs.y, fma_b(ph1, vs.y, h1 ^ 0x80008000u));
+            }
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const uint32_t ab = __byte_perm(vc.x, vc.y, j < 2 ? 0x5410 : 0x7632) >> (8 * (j & 1));
@@ -628,10 +644,15 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kOcc) k_kv4_attn(const __gr
 #pragma unroll
                 for (int i = 0; i < 4; i++) pr[i] = ex2(fmaf(sc[i], rs, -mref));
                 l += (pr[0] + pr[1]) + (pr[2] + pr[3]);
-                ph0 = pack_b(pr[0], pr[1]);
-                ph1 = pack_b(pr[2], pr[3]);
-                pl0 = pack_b(pr[0] - half_of(ph0, 0), pr[1] - half_of(ph0, 1));
-                pl1 = pack_b(pr[2] - half_of(ph1, 0), pr[3] - half_of(ph1, 1));
+                if constexpr (HILO) {
+                    p01 = pk(pr[0], pr[1]);
+                    p23 = pk(pr[2], pr[3]);
+                } else {
+                    ph0 = pack_b(pr[0], pr[1]);
+                    ph1 = pack_b(pr[2], pr[3]);
+                    pl0 = pack_b(pr[0] - half_of(ph0, 0), pr[1] - half_of(ph0, 1));
+                    pl1 = pack_b(pr[2] - half_of(ph1, 0), pr[3] - half_of(ph1, 1));
+                }
 #pragma unroll
                 for (int gr = 0; gr < G; gr++) value(rec, gr);
                 __syncwarp();
