@@ -22,9 +22,9 @@
 // codes in flight in registers), 16 the MMAs. S and P are double-buffered: while the softmax works on tile
 // j, the MMAs of P_{j-1} V and S_{j+1} run and K of tile j + 2 and V of tile j are converted.
 //
-// Measured: 512 tokens of 8 fp32 heads of 512 dimensions behind 15872 428 us (316 TFLOP/s
+// Measured: 512 tokens of 8 fp32 heads of 512 dimensions behind 15872 450 us (301 TFLOP/s
 // of the operator's, twice that on the tensor cores, which work on two terms of q and of
-// p); 2048 tokens of 256 dimensions behind 6144 289 us (417); 2048 tokens of 32 bf16 heads
+// p); 2048 tokens of 256 dimensions behind 6144 293 us (410); 2048 tokens of 32 bf16 heads
 // of 128 dimensions, 8 kv heads, 108 us (318). A tile takes 3.2 us at 512 dimensions, where
 // the MMAs need 1.4 and sending the halves of S (32 KB each way, st.async; plain remote
 // stores with one arrival a warp 522 us, sending before the maximum 463 us) bounds it; 2.1 us
@@ -69,9 +69,10 @@ struct Cfg {
     static constexpr int kV = kDc * 128;                     // V^T: rows are dimensions, 64 keys
     // The tensor cores truncate as they add up, 8 steps a tile: an error that grows with
     // the length of a run (fp32, 128 tiles: 2e-5 of the output, 4e-5 where values have one
-    // sign). So O is added to a sum in memory, in fp32, after every kRun tiles; 16-bit
-    // outputs round by more than that up to 256.
-    static constexpr int kRun = HILO ? 32 : 256;
+    // sign; after 32 tiles 5.5e-6 and 9e-6, after 16 3.3e-6 and 4.3e-6). So O is added to a
+    // sum in memory, in fp32, after every kRun tiles: 5 % of a chunk's time (32 tiles: 1 %).
+    // 16-bit outputs round by more than that up to 256.
+    static constexpr int kRun = HILO ? 16 : 256;
     static constexpr int kX = kCl > 1 ? kM * kT * 4 : 0;     // the other CTA's half of S
     static constexpr int kSmem = kQ * (HILO ? 2 : 1) + kK + kV + kX;
 };
@@ -275,6 +276,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
     int t0, t1;
     tiles_of(it, split, p.splits, t0, t1);
     const int nt = t1 - t0;
+    // O is summed up in memory before tiles first, first + kRun, ...; not by all CTAs at once,
+    // which took each 7 us (chunk of 512 tokens, 16 tiles: 474 us, now 450)
+    const int first = C::kRun - (nt > C::kRun ? id % C::kRun : 0);
+    auto turn_at = [&](int j) { return j >= first && (j - first) % C::kRun == 0; };
 
     if (tid == 0) {
         mbar_init(&kfull, kConvWarps);
@@ -454,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
 #pragma unroll
                         for (int i = 0; i < kT / 16; i++)
                             mma_f16_ta(tmem + kColO, tmem + kColP + b * 64 + half * 32 + i * 8, umma_desc(vb, i * 32),
-                                       kIdO, j % C::kRun || half || i);
+                                       kIdO, (j && !turn_at(j)) || half || i);
                     mma_commit(&odone[b]);
                 }
                 if (j + 2 < nt) {
@@ -760,7 +765,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
             pair[b][half][r] = mx;
             bar_sync(1 + quad, 64);
             mx = fmaxf(mx, pair[b][half ^ 1][r]) * rs;
-            const bool grow = mx > m + kSlack, turn = j > 0 && j % C::kRun == 0;
+            const bool grow = mx > m + kSlack, turn = turn_at(j);
             if (turn) {                                         // the run up to tile j - 1 is complete
                 wait(&odone[b ^ 1], (j - 1) >> 1);
                 tc_fence_after();
@@ -768,7 +773,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
                 float *acc = sums();
                 // Nothing but this thread touches its sums, so additions in memory have one
                 // order. The reference rarely moves once a few tiles are done.
-                const bool same = __all_sync(0xffffffffu, f == 1.0f), first = j == C::kRun;
+                const bool same = __all_sync(0xffffffffu, f == 1.0f);
 #pragma unroll 1
                 for (int c = half * (DC / 2); c < (half + 1) * (DC / 2); c += 32) {
                     int v[32];
@@ -779,7 +784,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
                         float4 *to = reinterpret_cast<float4 *>(acc + (c + x) * kM);
                         float4 y = make_float4(__int_as_float(v[x]), __int_as_float(v[x + 1]), __int_as_float(v[x + 2]),
                                                __int_as_float(v[x + 3]));
-                        if (first) __stcg(to, y);
+                        if (j == first) __stcg(to, y);
                         else if (same) red_add4(&to->x, y.x, y.y, y.z, y.w);
                         else {
                             const float4 z = __ldcg(to);
@@ -855,7 +860,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
 #pragma unroll
                 for (int x = 0; x < 32; x++) v[x] = 0;
             }
-            if (nt > C::kRun) {
+            if (nt > first) {
 #pragma unroll
                 for (int x = 0; x < 32; x += 4) {
                     const float4 y = __ldcg(reinterpret_cast<const float4 *>(acc + (c + x) * kM));
