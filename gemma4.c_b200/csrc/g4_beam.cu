@@ -34,8 +34,8 @@ G4_DEV uint64_t key_of(float x, uint32_t i) { return (uint64_t)order_f32(x) << 3
 // What a slice leaves: max, sum of its exponentials, then `beams` keys, best first
 // (0: the slice has no more values).
 struct SliceStat {
-    float max, m2;
-    double sum;      // of 2^(c x - m2)
+    float max;
+    double sum;      // of e^(x - max)
 };
 
 struct BeamArgs {
@@ -111,6 +111,10 @@ G4_DEV float ex2(float x) {
 // (4.5 TB/s), in bf16 the same. Measured beside it (with the merge, 35 us): 32 values a
 // thread and chunk 41 us, five CTAs an SM 37 us, two waves of shorter slices 37 us,
 // rings of 48 KB in shared memory filled by cp.async 39 us.
+// A slice whose first chunk is one value throughout (masked) has that value for its
+// threshold: more than kBuffer pass, and the slice is read again for every beam. 16 x 8
+// beams of 262144 with the first half masked 343 us; with 99 % masked here and there 37 us
+// (-inf) to 43 (-1e10).
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads, kOcc) k_beam_rows(BeamArgs a) {
     constexpr int N = Wide<T>::N, E = kChunk / kThreads, V = E / N;
@@ -137,19 +141,31 @@ __global__ void __launch_bounds__(kThreads, kOcc) k_beam_rows(BeamArgs a) {
         for (int e = 4; e < E; e++) m[e & 3] = fmaxf(m[e & 3], x[e]);
         return fmaxf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), -INFINITY);      // NaN: none
     };
-    // 2^(x c - m2) with c = log2 e rounded to fp32 and m2 = c max, rounded: what that
-    // leaves out is put right in the merge
+    // Up to kFar the sum is of 2^(c x - m2), one fma a value, with c = log2 e rounded to fp32
+    // and m2 = c tmax, rounded: at most 16 off, and put right when the threads join. A
+    // larger maximum (a mask of -1e10 or of the type's lowest value wherever no token of
+    // the thread is left) would make that factor overflow, or m2 itself: there the sum is of
+    // 2^(c (x - tmax)).
+    constexpr float kFar = 0x1p28f;
     float tmax = -INFINITY, m2 = 0.0f, sum = 0.0f;
+    auto near = [&](float m) { return fabsf(m) <= kFar; };
+    auto off = [&](float m, float c2) { return near(m) ? fmaf(-kC, m, c2) : 0.0f; };      // m2 - c m
     auto add = [&](float m) {
         if (m > tmax) {
             const float n2 = m * kC;
-            sum = tmax == -INFINITY ? 0.0f : sum * ex2(m2 - n2);
+            if (near(tmax) && near(m)) sum *= ex2(m2 - n2);
+            else if (tmax > -INFINITY) sum *= ex2(fmaf(tmax - m, kC, off(tmax, m2) - off(m, n2)));
             tmax = m;
             m2 = n2;
         }
         float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (near(tmax)) {
 #pragma unroll
-        for (int e = 0; e < E; e++) part[e & 3] += ex2(fmaf(x[e], kC, -m2));
+            for (int e = 0; e < E; e++) part[e & 3] += ex2(fmaf(x[e], kC, -m2));
+        } else if (tmax > -INFINITY) {
+#pragma unroll
+            for (int e = 0; e < E; e++) part[e & 3] += ex2((x[e] - tmax) * kC);
+        }
         sum += (part[0] + part[1]) + (part[2] + part[3]);
     };
     // the maxima of 32 groups of threads: the k-th largest is a threshold that at
@@ -240,7 +256,7 @@ __global__ void __launch_bounds__(kThreads, kOcc) k_beam_rows(BeamArgs a) {
             for (int e = 0; e < E; e++) {
                 const int i = index(base, e);
                 const float y = i < end ? (float)p[i] : -INFINITY;
-                if (y == y) sum += ex2(fmaf(y, kC, -m2));
+                if (y == y) sum += ex2(near(tmax) ? fmaf(y, kC, -m2) : (y - tmax) * kC);
             }
     }
 
@@ -250,8 +266,7 @@ __global__ void __launch_bounds__(kThreads, kOcc) k_beam_rows(BeamArgs a) {
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kThreads / 32; i++) bm = fmaxf(bm, wmax[i]);
-    const float b2 = bm == -INFINITY ? 0.0f : bm * kC;
-    double total = tmax == -INFINITY ? 0.0 : (double)sum * (double)ex2(m2 - b2);
+    double total = tmax == -INFINITY ? 0.0 : (double)sum * (double)ex2(fmaf(tmax - bm, kC, off(tmax, m2)));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     if (lane == 0) wsum[warp] = total;
@@ -259,7 +274,7 @@ __global__ void __launch_bounds__(kThreads, kOcc) k_beam_rows(BeamArgs a) {
     if (tid == 0) {
         double all = 0.0;
         for (int i = 0; i < kThreads / 32; i++) all += wsum[i];
-        a.stats[(long long)row * a.slices + slice] = {bm, b2, all};
+        a.stats[(long long)row * a.slices + slice] = {bm, all};
     }
     const int n = count;
     uint64_t *out = a.keys + ((long long)row * a.slices + slice) * a.beams;
@@ -317,7 +332,8 @@ G4_DEV bool better(const Cand &x, const Cand &y) {
 // One CTA per group. Candidates are few (beams per slice), so the same threshold
 // as in a slice leaves little more than `beams` of them, which rank one another.
 __global__ void __launch_bounds__(kMergeThreads) k_beam_merge(BeamArgs a) {
-    __shared__ double lse[kMaxBeams];       // of a live row
+    __shared__ double lsum[kMaxBeams];      // of a live row: log of the sum of e^(x - top)
+    __shared__ float top[kMaxBeams];
     __shared__ float cums[kMaxBeams];
     __shared__ int kind[kMaxBeams];         // 0 live, 1 all -inf, 2 finished
     __shared__ uint64_t gmax[32], b_score[kBuffer], b_at[kBuffer];
@@ -332,16 +348,16 @@ __global__ void __launch_bounds__(kMergeThreads) k_beam_merge(BeamArgs a) {
         float m = -INFINITY;
         for (int s = lane; s < a.slices; s += 32) m = fmaxf(m, st[s].max);
         m = warp_max(m);
-        // a slice's sum times 2^(m2 - c max) is the sum of e^((x - max) c ln 2)
         double sum = 0.0;
         for (int s = lane; s < a.slices; s += 32)
-            if (st[s].max > -INFINITY) sum += st[s].sum * exp2((double)st[s].m2 - (double)kC * (double)m);
+            if (st[s].max > -INFINITY) sum += st[s].sum * exp((double)st[s].max - (double)m);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == 0) {
             cums[r] = cum;
             kind[r] = cum - cum != 0.0f ? 1 : done ? 2 : m - m != 0.0f ? 1 : 0;
-            lse[r] = kind[r] == 0 ? (double)m + log(sum) : 0.0;
+            top[r] = m;
+            lsum[r] = kind[r] == 0 ? log(sum) : 0.0;
         }
     }
     __syncthreads();
@@ -352,7 +368,9 @@ __global__ void __launch_bounds__(kMergeThreads) k_beam_merge(BeamArgs a) {
         if (kind[r] == 0) {
             const uint64_t key = j < per_row - 1 ? a.keys[((long long)grp * a.beams + r) * a.slices * a.beams + j] : 0;
             if (key) {
-                x.score = order_f64((double)cums[r] + ((double)value_f32((uint32_t)(key >> 32)) - lse[r]));
+                // (the maximum first: beside one of 1e10 the logarithm would be lost)
+                x.score = order_f64((double)cums[r] +
+                                    (((double)value_f32((uint32_t)(key >> 32)) - (double)top[r]) - lsum[r]));
                 x.at = (uint64_t)r << 32 | (uint32_t)~(uint32_t)key;
             }
         } else if (j < few) {

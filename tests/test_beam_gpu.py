@@ -109,6 +109,93 @@ def test_masked_and_special_values(g4):
     check(g4, x, scores, np.array([[False, True, False, True]]), eos=3)
 
 
+def best(row, count):
+    """The `count` best tokens of a row and their log softmax in 64 bits, the maximum taken off
+    first: beside one of 1e10 the logarithm of the sum would be lost."""
+    x = row.double().cpu().numpy()
+    x = np.where(np.isnan(x), -np.inf, x)
+    d = x - x.max()
+    at = np.lexsort((np.arange(len(x)), -x))[:count]
+    return at, d[at] - np.log(np.exp(d).sum())
+
+
+def alone(g4, row):
+    """A row that has to win: as a search of its own, with one beam and with beams far behind it."""
+    vocab = row.shape[-1]
+    got = run(g4, row.reshape(1, vocab).contiguous(), np.array([[-1.5]]))
+    at, s = best(row, 1)
+    assert got[2].tolist() == [at.tolist()]
+    assert abs(got[0][0, 0] - (s[0] - 1.5)) <= 2.0 ** -24 * abs(s[0] - 1.5) + 2.0 ** -20
+    x = torch.zeros((4, vocab), dtype=row.dtype, device="cuda:0")
+    x[2] = row
+    got = run(g4, x, np.array([[-5000.0, -5000.0, 0.0, -5000.0]]))
+    at, s = best(row, 4)
+    n = int((s > -4000).sum())                          # the others come from the beams behind
+    assert n >= 1 and got[1][0, :n].tolist() == [2] * n and got[2][0, :n].tolist() == at[:n].tolist()
+    assert (got[1][0, n:] != 2).all()
+    assert (np.abs(got[0][0, :n] - s[:n]) <= 2.0 ** -24 * np.abs(s[:n]) + 2.0 ** -20).all()
+
+
+FAR = {"f32": (-3.4028234663852886e38, -1e30, -1e10, -3e9, -2.0 ** 28 - 32, -2.0 ** 28, 2.0 ** 28 + 32, 1e10, 3e38),
+       "bf16": (-3.3895313892515355e38, -1e30, -1e10, -3e9, 2.0 ** 28 + 2.0 ** 21, 3e38), "f16": (-65504.0, 65504.0)}
+
+
+@pytest.mark.parametrize("name,value", [(n, v) for n, vs in FAR.items() for v in vs])
+@pytest.mark.parametrize("vocab", [7, 5000, 70001])
+def test_far_logits(g4, name, value, vocab):
+    """Finite logits of any size (a vocabulary masked with the type's lowest value or -1e10):
+    rows of them alone, with one token left, with parts of the row left, and neighbouring values
+    that are still within a few units of each other. Each row is checked where it wins."""
+    dtype = TYPES[name]
+    rng = np.random.default_rng(vocab)
+    far = torch.full((vocab,), value, dtype=dtype, device="cuda:0")
+    live = torch.from_numpy(rng.standard_normal(vocab).astype(np.float32)).to(dtype).cuda()
+    alone(g4, far)
+    for keep in (slice(vocab // 2, vocab // 2 + 1), slice(0, vocab // 2), slice(vocab // 2, None)):
+        x = far.clone()
+        x[keep] = live[keep]
+        alone(g4, x)
+    x = far.clone()
+    x[::3] = torch.nextafter(far[0], torch.zeros_like(far[0]))
+    x[1::3] = torch.nextafter(x[0], torch.zeros_like(far[0]))
+    alone(g4, x)
+    x[vocab // 2] = float("nan")                        # summed up once more without it
+    alone(g4, x)
+    x = far.clone()
+    x[vocab // 3:] = float("-inf")
+    alone(g4, x)
+
+
+def test_far_logits_rise_and_fall(g4):
+    """Sizes that change from chunk to chunk of a slice: the running maximum crosses every form of the sum."""
+    steps = [-3.4028234663852886e38, -1e30, -1e10, -2.0 ** 28 - 32, -2.0 ** 28, -1e6, -3.0, 2.0, 1e6, 2.0 ** 28,
+             2.0 ** 28 + 32, 1e10, 3e38]
+    # 64 searches of 4 beams leave one slice of several chunks per row
+    for order in (steps, steps[::-1], steps[::2] + steps[1::2]):
+        row = torch.tensor(np.repeat(np.array(order, np.float32), 4096), device="cuda:0")
+        for last in range(1, len(order) + 1):
+            x = torch.zeros((4 * 64, last * 4096), device="cuda:0")
+            x[2::4] = row[:last * 4096]
+            got = run(g4, x, np.tile(np.array([[-5000.0, -5000.0, 0.0, -5000.0]]), (64, 1)))
+            top = row[:last * 4096].double()
+            want = -np.log(float((top - top.max()).exp().sum()))
+            assert (got[1][:, 0] == 2).all() and (got[2][:, 0] == int(top.argmax())).all(), (order, last)
+            assert (np.abs(got[0][:, 0] - want) <= 2.0 ** -24 * abs(want) + 2.0 ** -20).all(), (order, last)
+
+
+def test_special_rows_win(g4):
+    """Every kind of special row as the row that wins: few tokens left, NaN among them, one value."""
+    rng = np.random.default_rng(8)
+    inf, nan = float("inf"), float("nan")
+    x = torch.from_numpy(rng.standard_normal(5000).astype(np.float32)).cuda()
+    for change in (lambda r: r[10:].fill_(-inf), lambda r: r[:4990].fill_(-inf), lambda r: r[::3].fill_(nan),
+                   lambda r: r[5:].fill_(torch.finfo(torch.float32).min), lambda r: r[1:].fill_(nan)):
+        row = x.clone()
+        change(row)
+        for dtype in TYPES.values():
+            alone(g4, row.clamp(min=torch.finfo(dtype).min).where(row != -inf, row).to(dtype))
+
+
 def test_peaked_rows(g4):
     """One token holds nearly all probability; the others' order survives."""
     x = torch.full((2, 100000), -30.0, device="cuda:0")
