@@ -334,16 +334,19 @@ __global__ void __launch_bounds__(256) k_kv4_reorder(const __grid_constant__ Reo
     const int full = len >> a.page_shift, left = len & ((1 << a.page_shift) - 1);
     const bool moved = p != i && left > 0 && full < a.table_stride;
     const int *mine = a.table_in + (long long)i * a.table_stride, *from = a.table_in + (long long)p * a.table_stride;
+    const int src = moved ? from[full] : -1, dst = a.spare_in[i];
+    const bool src_ok = (unsigned)src < (unsigned)a.num_pages, dst_ok = (unsigned)dst < (unsigned)a.num_pages;
+    // A parent without a page there leaves nothing to copy: the spare page, whose old content
+    // would become keys, stays a spare one and the beam has no page either.
+    const bool none = moved && !src_ok && dst_ok;
     if (layer == a.layers) {
         int *out = a.table_out + (long long)i * a.table_stride;
         for (int j = threadIdx.x; j < a.table_stride; j += blockDim.x)
-            out[j] = j < full ? from[j] : j == full && moved ? a.spare_in[i] : mine[j];
-        if (threadIdx.x == 0) a.spare_out[i] = moved ? mine[full] : a.spare_in[i];
+            out[j] = j < full ? from[j] : j == full && moved ? (none ? src : dst) : mine[j];
+        if (threadIdx.x == 0) a.spare_out[i] = moved && !none ? mine[full] : dst;
         return;
     }
-    if (!moved) return;
-    const int src = from[full], dst = a.spare_in[i];
-    if ((unsigned)src >= (unsigned)a.num_pages || (unsigned)dst >= (unsigned)a.num_pages || src == dst) return;
+    if (!src_ok || !dst_ok || src == dst) return;
     const int hb = a.head_bytes[layer];
     const int n16 = ((left + kKv4Rec - 1) / kKv4Rec) * a.rec_bytes[layer] / 16;   // 16-byte pieces per head
     const uint8_t *s = a.pages[layer] + (long long)src * hb * a.heads[layer];

@@ -221,7 +221,10 @@ int g4_beam_select(int groups, int beams, int vocab, int type, const void *logit
  * page_size tokens) every beam has its own: a beam with another parent gets
  * its spare page, into which the records of 16 tokens that hold the parent's
  * tokens are copied in each of the `layers` caches (1..64, same page size and
- * count; one table for all), and its former page becomes its spare one.
+ * count; one table for all), and its former page becomes its spare one. Where the
+ * parent has no page there, the beam's entry becomes the parent's, so that its
+ * tokens are not seen either; the beam keeps its spare page, and its former page is
+ * in no table any more.
  * Entries after those stay the beam's own, so a beam needs its own page for
  * every page_size tokens it generates, and one to spare. Tables:
  * [groups * beams][table_stride], spare pages [groups * beams]; the outputs

@@ -675,3 +675,39 @@ def test_reorder_bad_pages(g4):
                        dev([n]).data_ptr(), table.data_ptr(), t_out.data_ptr(), 2, spare.data_ptr(), s_out.data_ptr())
         assert torch.equal(pool, before)
         assert s_out.tolist() == [77, -2]
+
+
+@pytest.mark.parametrize("missing", [-1, 77])
+def test_reorder_of_a_missing_page(g4, missing):
+    """The parent's part-full page is no page: its tokens are not seen by the child either,
+    whatever the child's spare page held before."""
+    page, hd, length = 16, 64, 20
+    rng = np.random.default_rng(3)
+    pool = dev(rng.integers(0, 256, (8, 1, 1, 17 * hd)), torch.uint8)
+    cache = g4.Kv4Cache(pool.data_ptr(), 8, page, 1, hd)
+    table, spare = dev([[0, missing, 5], [1, 2, 6], [3, 7, 6]]), dev([3, 4, 5])
+    off, start = dev([0, length, 2 * length, 3 * length]), dev([0, 0, 0])
+    k = tensors(rng, 3 * length, 1, hd, torch.float32)
+    batch = g4.Kv4Batch(3, 3 * length, off.data_ptr(), start.data_ptr(), table.data_ptr(), 3)
+    g4.kv4_write(cache, batch, 0, k.data_ptr(), k.stride(0), k.data_ptr(), k.stride(0))
+    before = pool.clone()
+    parents, lengths = dev([0, 0, 1]), dev([length])
+    t_out, s_out = torch.empty_like(table), torch.empty_like(spare)
+    g4.kv4_reorder(g4.kv4_caches([cache]), 1, 3, parents.data_ptr(), lengths.data_ptr(), table.data_ptr(),
+                   t_out.data_ptr(), 3, spare.data_ptr(), s_out.data_ptr())
+    assert t_out.tolist() == [[0, missing, 5], [0, missing, 6], [1, 5, 6]] and s_out.tolist() == [3, 4, 7]
+    want = before.clone()
+    want[5] = before[2]                                # only the beam whose parent has its page copies one
+    assert torch.equal(pool, want)
+    # the child sees what the parent sees: the 16 keys of the full page
+    q = tensors(rng, 1, 1, hd, torch.float32).expand(3, 1, hd).contiguous()
+    out = torch.empty_like(q)
+    step, at = dev([0, 1, 2, 3]), dev([length - 1] * 3)
+    b = g4.Kv4Batch(3, 3, step.data_ptr(), at.data_ptr(), t_out.data_ptr(), 3)
+    ws = torch.empty(g4.kv4_attention_workspace(cache, b, 0, 1), dtype=torch.uint8, device="cuda:0")
+    g4.kv4_attention(cache, b, 0, 1, q.data_ptr(), hd, out.data_ptr(), hd, 0.1, 0, ws.data_ptr(), ws.numel())
+    kk = ref.stored(as64(k[:16]))
+    want, mag, delta, n = ref.attention(as64(q)[0], kk, kk, 15, 0.1, 0)
+    tol = ref.tolerance(want, mag, delta, n, 2.0 ** -23)
+    assert (np.abs(as64(out)[0] - want) <= tol).all() and torch.equal(out[0], out[1])
+    assert not torch.equal(out[0], out[2])
