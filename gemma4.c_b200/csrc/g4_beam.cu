@@ -493,8 +493,11 @@ extern "C" {
 
 uint64_t g4_beam_workspace(int groups, int beams, int vocab) {
     if (!sizes_ok(groups, beams, vocab)) return 0;
-    const uint64_t rows = (uint64_t)(groups ? groups : 1) * beams;
-    return rows * slices_per_row(rows, vocab) * (sizeof(SliceStat) + beams * sizeof(uint64_t));
+    // What the largest of all calls of at most these sizes takes: rows that are split have at
+    // most kOcc * kSms slices together (of 100000 values, 64 rows have 576 and 128 rows 512).
+    const uint64_t rows = (uint64_t)(groups ? groups : 1) * beams, chunks = ((uint64_t)vocab + kChunk - 1) / kChunk,
+                   split = rows * chunks < kOcc * kSms ? rows * chunks : kOcc * kSms;
+    return (rows > split ? rows : split) * (sizeof(SliceStat) + beams * sizeof(uint64_t));
 }
 
 int g4_beam_select(int groups, int beams, int vocab, int type, const void *logits, int64_t logits_stride,

@@ -209,7 +209,8 @@ int g4_kv4_attention(const g4_kv4_cache *cache, const g4_kv4_batch *batch, int t
  * not overlapping the inputs; parents count within the group, out_finished is
  * the parent's flag or token == eos. The softmax's sum and the scores are
  * joined in fp64. workspace: g4_beam_workspace bytes, 16-byte aligned, any
- * content, scratch of this call alone. */
+ * content, scratch of this call alone; what it says for some groups, beams and
+ * vocab is enough for every call with as many or fewer of each. */
 uint64_t g4_beam_workspace(int groups, int beams, int vocab);
 int g4_beam_select(int groups, int beams, int vocab, int type, const void *logits, int64_t logits_stride,
                    const float *scores, const unsigned char *finished, int eos, float *out_scores, int *parents,

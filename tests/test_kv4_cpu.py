@@ -93,6 +93,27 @@ def test_beam_refusals(g4):
             g4.beam_workspace(*bad)
 
 
+def test_beam_workspace_serves_every_smaller_call(g4):
+    """A buffer sized for the largest search is enough when searches end, beams are fewer or the
+    vocabulary is shorter, and it holds what a call of those sizes fills: 16 bytes and a
+    key of 8 per beam for every slice of a row, as many slices as four CTAs on each of
+    148 SMs leave it."""
+    sizes = [(g, w, v) for g in (1, 2, 3, 7, 16, 64, 65, 200) for w in (1, 2, 4, 5, 8, 31, 32)
+             for v in (1, 4096, 4097, 50001, 100000, 262144)]
+    need = {s: g4.beam_workspace(*s) for s in sizes}
+    for s, n in need.items():
+        rows, chunks = s[0] * s[1], -(-s[2] // 4096)
+        slices = 592 // rows
+        per = chunks if slices <= 1 else -(-chunks // slices)
+        assert n >= rows * -(-chunks // per) * (16 + 8 * s[1]), s
+        smaller = [m for t, m in need.items() if all(a <= b for a, b in zip(t, s))]
+        assert max(smaller) == n, s
+    refused = g4.load().g4_beam_select
+    n = g4.beam_workspace(3, 4, 262144)
+    args = (P, 262144, P, None, -1, P, P, P, None, P)
+    assert refused(3, 4, 262144, 0, *args, n - 1, None) == -1
+
+
 def test_reorder_refusals(g4):
     f = g4.load().g4_kv4_reorder
     far = P + (1 << 20)
