@@ -119,6 +119,20 @@ cudaError_t g4_launch_kv4_attention(const Kv4View &c, int type, int q_heads, con
                                     void *out, long long out_stride, float scale, int window, void *ws,
                                     cudaStream_t st);
 size_t g4_kv4_attention_ws(const Kv4View &c, int type, int q_heads);
+// Many query rows per sequence and kv head go to the tcgen05 tiles of 128 rows, few to
+// tiles of 8 (g4_kv4_attn.cu), whose time grows with the rows while the other's starts at 33
+// (256 dimensions) to 43 us (512) for a context of 4000. Measured on either side, us of the small
+// and the large tiles: 16 sequences, 512 dimensions, 8 tokens x 8 heads on average 71 / 120, 16 tokens
+// 127 / 124, 33 tokens 236 / 176; 256 dimensions, 16 tokens 74 / 69; 128 dimensions, 8 kv heads
+// of 4, 16 tokens 134 / 169, 33 tokens 250 / 205. Fewer than four sequences and heads of many
+// dimensions leave the large tiles less to share out: one sequence and kv head of 512
+// dimensions, 64 tokens x 8 heads 47 / 50, 128 tokens 80 / 53; of 256 dimensions 35 / 37 and
+// 51 / 36. Hence their own bound.
+constexpr int kManyRows = 112, kManyRowsAlone = 576;
+inline bool many_rows(const Kv4View &c, int q_heads) {
+    const long long from = c.hd >= 256 && (long long)c.n * c.kv_heads < 4 ? kManyRowsAlone : kManyRows;
+    return (long long)c.rows * (q_heads / c.kv_heads) >= from * c.n;
+}
 // g4_kv4_prompt.cu: the same for many query rows per sequence
 size_t kv4_prompt_ws(const Kv4View &c, int type, int q_heads);
 cudaError_t kv4_launch_prompt(const Kv4View &c, int type, int q_heads, const void *q, long long q_stride, void *out,

@@ -42,6 +42,8 @@
 // one in 378: 128 MMAs and the ANDs, shifts and adds of the codes share the issue. Not better:
 // two warps a record, Q K of the next record beside P V, separate accumulators for the
 // high and low halves.
+#include <algorithm>
+
 #include <cuda_runtime.h>
 
 #include "g4_kv4.cuh"
@@ -868,24 +870,12 @@ size_t ws_bytes() {
 
 }  // namespace
 
-// Many query rows per sequence and kv head go to the tcgen05 tiles of 128 rows, few to
-// this file's tiles of 8, whose time grows with the rows while the other's starts at 33
-// (256 dimensions) to 43 us (512) for a context of 4000. Measured on either side, us here
-// and there: 16 sequences, 512 dimensions, 8 tokens x 8 heads on average 71 / 120, 16 tokens
-// 127 / 124, 33 tokens 236 / 176; 256 dimensions, 16 tokens 74 / 69; 128 dimensions, 8 kv heads
-// of 4, 16 tokens 134 / 169, 33 tokens 250 / 205. Fewer than four sequences and heads of many
-// dimensions leave the large tiles less to share out: one sequence and kv head of 512
-// dimensions, 64 tokens x 8 heads 47 / 50, 128 tokens 80 / 53; of 256 dimensions 35 / 37 and
-// 51 / 36. Hence their own bound.
-static bool many_rows(const Kv4View &c, int q_heads) {
-    const long long from = c.hd >= 256 && (long long)c.n * c.kv_heads < 4 ? 576 : 112;
-    return (long long)c.rows * (q_heads / c.kv_heads) >= from * c.n;
-}
-
 size_t g4_kv4_attention_ws(const Kv4View &c, int type, int q_heads) {
     if (c.n == 0) return 16;
-    if (many_rows(c, q_heads)) return kv4_prompt_ws(c, type, q_heads);
-    return c.hd == 64 ? ws_bytes<64>() : c.hd == 128 ? ws_bytes<128>() : c.hd == 256 ? ws_bytes<256>() : ws_bytes<512>();
+    // enough for every call of fewer rows, sequences or pages too, whichever kernel that takes
+    const size_t few =
+        c.hd == 64 ? ws_bytes<64>() : c.hd == 128 ? ws_bytes<128>() : c.hd == 256 ? ws_bytes<256>() : ws_bytes<512>();
+    return std::max(few, kv4_prompt_ws(c, type, q_heads));
 }
 
 cudaError_t g4_launch_kv4_attention(const Kv4View &c, int type, int q_heads, const void *q, long long q_stride,

@@ -29,6 +29,7 @@
 // the MMAs need 1.4 and sending the halves of S (32 KB each way, st.async; plain remote
 // stores with one arrival a warp 522 us, sending before the maximum 463 us) bounds it; 2.1 us
 // at 256, where MMAs of 64 columns (48 clocks against 32 for their share) bound it.
+#include <algorithm>
 #include <atomic>
 
 #include <cuda_runtime.h>
@@ -960,7 +961,7 @@ int ranges(const Kv4View &c, long long items, long long tiles) {
     }
     return n;
 }
-// The workspace is sized without the window, which can only make the ranges fewer.
+// (The window can only make the ranges fewer: the workspace is sized without it.)
 void plan(const Kv4View &c, unsigned group, int window, int *tokens, int *slots, int *splits) {
     *tokens = kM / (int)group;
     *slots = c.rows / *tokens + c.n;
@@ -1015,12 +1016,29 @@ cudaError_t launch_hd(const PromptP &p, cudaStream_t st) {
 
 }  // namespace
 
+// Bytes that any call of at most c.rows rows, c.n sequences and c.table_stride pages takes, of
+// those that come here: plan() gives fewer rows more key ranges of a tile (bounded by 4 room /
+// items in ranges()), so every number of row tiles that may be cut is looked at.
 size_t kv4_prompt_ws(const Kv4View &c, int type, int q_heads) {
-    int tokens, slots, splits;
-    plan(c, q_heads / c.kv_heads, 0, &tokens, &slots, &splits);
+    const int group = q_heads / c.kv_heads, tokens = kM / group;
+    const long long room = kSms / (c.hd > 256 ? 2 : 1), all = (c.rows + tokens - 1) / tokens,
+                    tiles = (((long long)c.table_stride << c.page_shift) + kT - 1) / kT;
     const int run = type == G4_TYPE_F32 ? Cfg<64, true>::kRun : Cfg<64, false>::kRun;
-    const bool runs = ((long long)c.table_stride << c.page_shift) > run * kT;      // of tiles, to be summed up
-    return splits == 1 && !runs ? 16 : (size_t)slots * c.kv_heads * splits * kM * (c.hd + 2) * sizeof(float);
+    long long most = 0;
+    for (long long t = 1; t <= all; t++) {
+        long long splits = 4 * room / (t * c.kv_heads);
+        splits = std::min(std::min(splits, 32ll), tiles);
+        if (splits < 2) {
+            t = all;                                            // not cut: the most rows need most
+            splits = tiles > run ? 1 : 0;                       // of tiles, to be summed up
+        }
+        Kv4View v = c;                                          // the most sequences that make it many rows
+        v.rows = (int)std::min<long long>(t * tokens, c.rows);
+        v.n = (int)std::min<long long>(c.n, (long long)v.rows * group / kManyRows);
+        if (v.n > 0 && !many_rows(v, q_heads)) v.n = (int)std::min<long long>(c.n, (long long)v.rows * group / kManyRowsAlone);
+        if (v.n > 0) most = std::max(most, (v.rows / tokens + v.n) * splits);
+    }
+    return (size_t)most * c.kv_heads * kM * (c.hd + 2) * sizeof(float);
 }
 
 cudaError_t kv4_launch_prompt(const Kv4View &c, int type, int q_heads, const void *q, long long q_stride, void *out,

@@ -191,7 +191,8 @@ int g4_kv4_read(const g4_kv4_cache *cache, const g4_kv4_batch *batch, int type, 
  * dimensions. A wait inside a kernel that runs out (2 s) makes its rows NaN too.
  * `workspace` (g4_kv4_attention_workspace bytes, 16-byte aligned, any content)
  * is scratch of this call alone: calls that may overlap on the GPU (other
- * streams, other captured graphs) need their own. */
+ * streams, other captured graphs) need their own. What it says for some n, rows
+ * and table_stride is enough for every call with as many or fewer of each. */
 uint64_t g4_kv4_attention_workspace(const g4_kv4_cache *cache, const g4_kv4_batch *batch, int type, int q_heads);
 int g4_kv4_attention(const g4_kv4_cache *cache, const g4_kv4_batch *batch, int type, int q_heads, const void *q,
                      int64_t q_stride, void *out, int64_t out_stride, float scale, int window, void *workspace,

@@ -75,6 +75,42 @@ def test_attention_refusals(g4):
     assert g4.kv4_attention_workspace(cache(g4), batch(g4), 0, 8) > 0
 
 
+def prompt_bytes(hd, kv, heads, f32, n, rows, length):
+    """What the tiles of 128 rows fill for such a call: per row tile and kv head, for as many key
+    ranges as the rounds of the grid ask for, an output of 128 rows, their maxima and sums."""
+    group, room = heads // kv, 74 if hd > 256 else 148
+    tokens = 128 // group
+    items, tiles = -(-rows // tokens) * kv, -(-length // 64)
+    best, splits = None, 1
+    for s in range(1, min(32, tiles) + 1):
+        if s > 1 and items * s > 4 * room:
+            break
+        cost = -(-items * s // room) * (tiles / s + 3) + (items * s * hd / 20000 if s > 1 else 0)
+        if best is None or cost < 0.97 * best:
+            best, splits = cost, s
+    if splits == 1 and tiles <= (16 if f32 else 256):
+        return 0
+    return (rows // tokens + n) * kv * splits * 128 * (hd + 2) * 4
+
+
+@pytest.mark.parametrize("hd,kv,heads", [(64, 1, 8), (128, 8, 32), (128, 2, 10), (256, 1, 8), (512, 1, 8), (512, 2, 4)])
+@pytest.mark.parametrize("kind", [0, 1])
+def test_attention_workspace_serves_every_smaller_call(g4, kind, hd, kv, heads):
+    """A buffer sized for the longest prompt, the most sequences and the longest table is enough
+    for every decode step, shorter prompt and table, and holds what their plan fills."""
+    sizes = [(n, rows, stride) for n in (1, 2, 5, 16, 64) for rows in (1, 8, 60, 63, 70, 75, 100, 512, 513, 4096, 20000)
+             for stride in (1, 16, 17, 256, 2048)]
+    c = cache(g4, kv_heads=kv, head_dim=hd)
+    need = {s: g4.kv4_attention_workspace(c, batch(g4, n=s[0], rows=s[1], table_stride=s[2]), kind, heads)
+            for s in sizes}
+    slots = {64: 592, 128: 592, 256: 592, 512: 296}[hd] * 8 * (hd + 2) * 4
+    for s, b in need.items():
+        assert b >= slots, s                            # the few rows' partial outputs, two for every CTA
+        if s[1] * (heads // kv) >= (576 if hd >= 256 and s[0] * kv < 4 else 112) * s[0]:
+            assert b >= prompt_bytes(hd, kv, heads, kind == 0, s[0], s[1], s[2] * 64), s
+        assert b == max(m for t, m in need.items() if all(x <= y for x, y in zip(t, s))), s
+
+
 def test_beam_refusals(g4):
     f = g4.load().g4_beam_select
 

@@ -711,3 +711,23 @@ def test_reorder_of_a_missing_page(g4, missing):
     tol = ref.tolerance(want, mag, delta, n, 2.0 ** -23)
     assert (np.abs(as64(out)[0] - want) <= tol).all() and torch.equal(out[0], out[1])
     assert not torch.equal(out[0], out[2])
+
+
+@pytest.mark.parametrize("hd,kv,heads,name", [(512, 1, 8, "f32"), (128, 4, 16, "bf16")])
+def test_attention_in_a_workspace_of_the_largest_call(g4, hd, kv, heads, name):
+    """One buffer, sized for the largest call, serves chunks, single tokens and shorter tables
+    with the bits that they have in their own; nothing behind what a call asked for is touched."""
+    rng = np.random.default_rng(12)
+    big = Setup(g4, [(0, 600)] * 3, kv, hd, 64, stride=64)
+    n = g4.kv4_attention_workspace(big.cache, big.batch, kind_of(g4, name), heads)
+    ws = torch.empty(n + 4096, dtype=torch.uint8, device="cuda:0")
+    for spans, stride in (([(900, 1)], None), ([(2900, 70)], None), ([(100, 90)], None), ([(50, 1), (700, 300), (3, 1)], 64),
+                          ([(0, 500)] * 3, 64)):
+        s = Setup(g4, spans, kv, hd, 64, stride=stride)
+        q, want = check_attention(g4, s, heads, name, 0.1, 0, rng)
+        need = g4.kv4_attention_workspace(s.cache, s.batch, kind_of(g4, name), heads)
+        assert need <= n
+        ws.fill_(0x5A)
+        out = torch.empty_like(want)
+        s.attend(q, out, kind_of(g4, name), 0.1, 0, ws=ws[:n])
+        assert torch.equal(out, want) and (ws[need:] == 0x5A).all()
