@@ -6,6 +6,8 @@
 // in bf16 written and read back 79 us (360 MB, 4.6 TB/s: finding a tile's rows and page is
 // a chain of loads before each 16 tokens), 64 rows of 256 in fp32 6 us; reordering 16 x 8
 // beams in 15 layers 15 us (64 MB, 4.3 TB/s), 4 beams in 12 layers 2.6 us.
+#include <atomic>
+
 #include <cuda_runtime.h>
 
 #include "g4_kv4.cuh"
@@ -359,6 +361,8 @@ __global__ void __launch_bounds__(256) k_kv4_reorder(const __grid_constant__ Reo
     }
 }
 
+std::atomic<int> g_starve{0};       // g4_test_kv4_attention_starve
+
 bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 bool aligned4(const void *p) { return ((uintptr_t)p & 3) == 0; }
 
@@ -512,8 +516,14 @@ int g4_kv4_attention(const g4_kv4_cache *cache, const g4_kv4_batch *batch, int t
         !dev.holds(workspace))
         return G4_ERR_INVALID;
     const cudaError_t e = g4_launch_kv4_attention(c, type, q_heads, q, q_stride, out, out_stride, scale, window,
-                                                  workspace, (cudaStream_t)stream);
+                                                  workspace, g_starve.exchange(0), (cudaStream_t)stream);
     return e == cudaSuccess ? G4_OK : G4_ERR_CUDA;
+}
+
+int g4_test_kv4_attention_starve(int what) {
+    if (what < 0 || what > 2) return G4_ERR_INVALID;
+    g_starve = what;
+    return G4_OK;
 }
 
 int g4_kv4_reorder(const g4_kv4_cache *caches, int layers, int groups, int beams, const int *parents,

@@ -116,8 +116,8 @@ class DeviceOf {
 };
 
 cudaError_t g4_launch_kv4_attention(const Kv4View &c, int type, int q_heads, const void *q, long long q_stride,
-                                    void *out, long long out_stride, float scale, int window, void *ws,
-                                    cudaStream_t st);
+                                    void *out, long long out_stride, float scale, int window, void *ws, int starve,
+                                    cudaStream_t st);      // starve: g4_test_kv4_attention_starve
 size_t g4_kv4_attention_ws(const Kv4View &c, int type, int q_heads);
 // Many query rows per sequence and kv head go to the tcgen05 tiles of 128 rows, few to
 // tiles of 8 (g4_kv4_attn.cu), whose time grows with the rows while the other's starts at 33
@@ -136,4 +136,4 @@ inline bool many_rows(const Kv4View &c, int q_heads) {
 // g4_kv4_prompt.cu: the same for many query rows per sequence
 size_t kv4_prompt_ws(const Kv4View &c, int type, int q_heads);
 cudaError_t kv4_launch_prompt(const Kv4View &c, int type, int q_heads, const void *q, long long q_stride, void *out,
-                              long long out_stride, float scale, int window, void *ws, cudaStream_t st);
+                              long long out_stride, float scale, int window, void *ws, int starve, cudaStream_t st);

@@ -366,7 +366,8 @@ G4_DEV void next_item(const AttnP &p, Walk &w, Item &out) {
     out = it;
 }
 
-template <int HD, bool HILO>
+// STARVE: the test aid g4_test_kv4_attention_starve.
+template <int HD, bool HILO, bool STARVE>
 __global__ void __launch_bounds__(kThreads, Cfg<HD>::kOcc) k_kv4_attn(const __grid_constant__ AttnP p) {
     using C = Cfg<HD>;
     constexpr int G = C::G, REC = C::kRec, ST = C::kStages;
@@ -451,7 +452,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kOcc) k_kv4_attn(const __gr
             const uint8_t *src = (const uint8_t *)__shfl_sync(0xffffffffu, addr, k & 31);
             const int st = k % ST;
             there = src ? there | 1u << st : there & ~(1u << st);
-            if (src && lane == 0) {
+            if (src && lane == 0 && !(STARVE && blockIdx.x == 0 && stream == 0)) {
                 mbar_arrive_expect_tx(&full[stream][st], REC);
                 bulk_load(my_ring + st * REC, src, REC, &full[stream][st]);
             }
@@ -836,19 +837,20 @@ __global__ void __launch_bounds__(kJoinThreads) k_kv4_attn_join(const __grid_con
     }
 }
 
-template <int HD, bool HILO>
+template <int HD, bool HILO, bool STARVE = false>
 cudaError_t launch_stream(const AttnP &p, cudaStream_t st) {
     using C = Cfg<HD>;
+    constexpr auto kernel = k_kv4_attn<HD, HILO, STARVE>;
     const int smem = C::kRing + (HILO ? 2 : 1) * C::kQ + C::G * 32;
-    cudaError_t e = g4_smem_optin((const void *)k_kv4_attn<HD, HILO>, smem);
+    cudaError_t e = g4_smem_optin((const void *)kernel, smem);
     if (e != cudaSuccess) return e;
-    e = g4_launch(k_kv4_attn<HD, HILO>, dim3(C::kCtas), dim3(kThreads), (size_t)smem, st, true, p);
+    e = g4_launch(kernel, dim3(C::kCtas), dim3(kThreads), (size_t)smem, st, true, p);
     if (e != cudaSuccess || p.whole) return e;
     return g4_launch(k_kv4_attn_join<HD>, dim3(C::kCtas - 1), dim3(kJoinThreads), 0, st, true, p);
 }
 
 template <int HD>
-cudaError_t launch_hd(AttnP &p, cudaStream_t st) {
+cudaError_t launch_hd(AttnP &p, int starve, cudaStream_t st) {
     // Items of few records, not more of them than CTAs: a CTA has an item for itself, and the
     // second kernel is saved. One token of 8 heads and a window of 512 tokens (33 records), us
     // cut and whole: 64 dimensions, 1 / 64 / 128 sequences 9.7 / 7.7, 12.5 / 9.4, 16.4 / 9.8; 256
@@ -860,6 +862,9 @@ cudaError_t launch_hd(AttnP &p, cudaStream_t st) {
                     tiles = (long long)p.c.rows * p.group / kRows + p.c.n;
     p.whole = seen <= Cfg<HD>::kWhole * kKv4Rec && tiles * p.c.kv_heads <= Cfg<HD>::kCtas;
     p.stats = p.slots + (size_t)2 * Cfg<HD>::kCtas * Cfg<HD>::kSlot;
+    if constexpr (HD >= 256)
+        if (starve == 1 && p.type == G4_TYPE_F32) return launch_stream<HD, true, true>(p, st);
+    if (starve) return cudaErrorNotSupported;
     return p.type == G4_TYPE_F32 ? launch_stream<HD, true>(p, st) : launch_stream<HD, false>(p, st);
 }
 
@@ -879,10 +884,10 @@ size_t g4_kv4_attention_ws(const Kv4View &c, int type, int q_heads) {
 }
 
 cudaError_t g4_launch_kv4_attention(const Kv4View &c, int type, int q_heads, const void *q, long long q_stride,
-                                    void *out, long long out_stride, float scale, int window, void *ws,
+                                    void *out, long long out_stride, float scale, int window, void *ws, int starve,
                                     cudaStream_t st) {
     if (many_rows(c, q_heads))
-        return kv4_launch_prompt(c, type, q_heads, q, q_stride, out, out_stride, scale, window, ws, st);
+        return kv4_launch_prompt(c, type, q_heads, q, q_stride, out, out_stride, scale, window, ws, starve, st);
     AttnP p;
     p.c = c;
     p.type = type;
@@ -894,8 +899,8 @@ cudaError_t g4_launch_kv4_attention(const Kv4View &c, int type, int q_heads, con
     p.scale = scale;
     p.window = window;
     p.slots = (float *)ws;
-    if (c.hd == 64) return launch_hd<64>(p, st);
-    if (c.hd == 128) return launch_hd<128>(p, st);
-    if (c.hd == 256) return launch_hd<256>(p, st);
-    return launch_hd<512>(p, st);
+    if (c.hd == 64) return launch_hd<64>(p, starve, st);
+    if (c.hd == 128) return launch_hd<128>(p, starve, st);
+    if (c.hd == 256) return launch_hd<256>(p, starve, st);
+    return launch_hd<512>(p, starve, st);
 }

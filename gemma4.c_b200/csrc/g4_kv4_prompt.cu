@@ -89,6 +89,7 @@ struct PromptP {
     long long q_stride, out_stride;
     float scale;
     int window;
+    int starve;                    // of a STARVE kernel: 1 K of block 0 is never announced, 2 a wait there counts as run out
     float *parts, *stats;          // [slots][kv heads][splits][HD / 4][128][4], [..][2][128]
 };
 
@@ -130,6 +131,9 @@ G4_DEV void remote_store4(uint32_t addr, float x, float y, float z, float w, uin
 }
 G4_DEV void remote_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+G4_DEV void remote_store(uint32_t addr, int x) {
+    asm volatile("st.relaxed.cluster.shared::cluster.s32 [%0], %1;" ::"r"(addr), "r"(x) : "memory");
 }
 G4_DEV bool wait_cluster(uint64_t *bar, uint32_t parity) {       // bounded, like mbar_wait
     const uint64_t t0 = g4_globaltimer();
@@ -245,7 +249,8 @@ G4_DEV uint32_t value2(uint32_t x, uint32_t mask, uint32_t s, uint32_t off) { re
 G4_DEV float bound(float f) { return f > 4080.0f ? 4080.0f : f < -4080.0f ? -4080.0f : f; }
 constexpr uint32_t kLoMask = 0x00780078u, kHiMask = 0x07800780u;
 
-template <int HD, bool HILO>
+// STARVE: the test aid g4_test_kv4_attention_starve.
+template <int HD, bool HILO, bool STARVE>
 __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constant__ PromptP p) {
     using C = Cfg<HD, HILO>;
     constexpr int G = C::G, HG = HD / kKv4Group, DC = C::kDc, CL = C::kCl;
@@ -434,12 +439,23 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
     const int ka = k_top ? min(max(11 - ((int)(k_top >> 7) - 127), -100), 113) : 0;
     const int va = v_top ? min(max(11 - ((int)(v_top >> 7) - 127), -100), 113) : 0;
 
-    bool lost = false;                                          // a wait ran out: no more waits, the output is NaN
+    // A wait ran out: this thread waits no more, and the rows of both CTAs are NaN, whose
+    // scores are made of both halves.
+    bool lost = false;
+    auto fail = [&]() {
+        lost = true;
+        failed = 1;
+        if constexpr (CL > 1) remote_store(rank_addr(smem_u32(&failed), rank ^ 1), 1);
+    };
     auto wait = [&](uint64_t *bar, int phase) {
-        if (!lost && !mbar_wait(bar, phase & 1, nullptr, 0)) {
-            lost = true;
-            failed = 1;
-        }
+        if (!lost && !mbar_wait(bar, phase & 1, nullptr, 0)) fail();
+    };
+    // All warps of the row tile, when every product is done and nothing is on its way between
+    // the CTAs any more: from here on `failed` says what it will say.
+    auto meet = [&]() {
+        __syncwarp();
+        if constexpr (CL > 1) cluster_sync();
+        else __syncthreads();
     };
 
     if (warp == kSoftWarps + kConvWarps) {
@@ -476,12 +492,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
                     mma_commit(&sfull[j & 1]);
                 }
             }
-            if (lost) {                                         // no MMA is left when TMEM is freed
-                mma_commit(&ended);
-                mbar_wait(&ended, 0, nullptr, 0);
-            }
+            mma_commit(&ended);                                 // no MMA is left when TMEM is freed
+            if (!mbar_wait(&ended, 0, nullptr, 0)) fail();
         }
-        __syncwarp();
+        meet();
     } else if (warp >= kSoftWarps) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kConvRegs));
         // ---- conversion: this warp's record of each tile, its groups g0, g0 + 2, ... ----
@@ -553,6 +567,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
             }
             fence_async();
             __syncwarp();
+            if (STARVE && blockIdx.x == 0) {
+                if (p.starve == 1) return;
+                if (p.starve == 2 && warp == kSoftWarps) fail();
+            }
             if (lane == 0) mbar_arrive(&kfull);
         };
         // NaN among the values of tile j: remembered by key, the operand is 0
@@ -668,6 +686,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
             page = page_of(j + 4);
             if (j + 3 < nt) fetch_k(r2);
         }
+        meet();
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
         // ---- softmax: threads (r, half) take keys 32 half .. + 31 of row r ----
@@ -693,10 +712,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
         // this CTA's half of S of a tile to the other CTA: on its way while the tile before
         // it is worked on
         const int x0 = (half * (kH / 4)) * kM + r;
+        // The warps of the pair go on or give up together: one that is lost sends nothing more and
+        // frees nothing, so that the other's waits run out too.
         auto send = [&](int j) {
             wait(&sfull[j & 1], j >> 1);
             tc_fence_after();
-            if (j > 0 && !lost && !wait_cluster(&xfree[warp], (j - 1) & 1)) lost = true, failed = 1;
+            if (j > 0 && !lost && !wait_cluster(&xfree[warp], (j - 1) & 1)) fail();
+            if (__any_sync(0xffffffffu, lost)) {
+                if (!lost) fail();
+                return;
+            }
 #pragma unroll
             for (int c = 0; c < kH; c += 16) {
                 int v[16];
@@ -717,7 +742,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
             if constexpr (CL == 1) {
                 wait(&sfull[b], j >> 1);
                 tc_fence_after();
-            } else if (!lost && !wait_cluster(&xfull[warp], j & 1)) lost = true, failed = 1;
+            } else if (!lost && !wait_cluster(&xfull[warp], j & 1)) fail();
             {
                 int v[kH];
                 tmem_ld32(lanes + kColS + b * kT + half * kH, v);
@@ -735,8 +760,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
                 }
             }
             if constexpr (CL > 1) {
-                __syncwarp();
-                if (lane == 0) remote_arrive(peer_free);
+                if (__any_sync(0xffffffffu, lost)) lost = true;
+                else if (lane == 0) remote_arrive(peer_free);
             }
             const int key0 = (t0 + j) * kT + half * kH;
             const bool gap0 = missing[j & 3][2 * half] == j + 1, gap1 = missing[j & 3][2 * half + 1] == j + 1;
@@ -835,6 +860,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
             if (lane == 0) mbar_arrive(&pfull[b]);
         }
         if (nt > 0) wait(&odone[(nt - 1) & 1], (nt - 1) >> 1);
+        // what the other CTA may have sent is still on its way: whichever phase is not complete
+        if (CL > 1 && lost)
+            for (int i = 0; i < 2; i++) wait_cluster(&xfull[warp], i);
+        meet();
         tc_fence_after();
         // ---- output: each thread of a row half of the dimensions ----
         pair[0][half][r] = l;
@@ -887,8 +916,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
         }
     }
     tc_fence_before();
-    if constexpr (CL > 1) cluster_sync();                       // the other CTA may still read or signal here
-    else __syncthreads();
+    __syncthreads();
     if (warp == kSoftWarps + kConvWarps) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
@@ -977,15 +1005,16 @@ void plan(const Kv4View &c, unsigned group, int window, int *tokens, int *slots,
     }
 }
 
-template <int HD, bool HILO>
+template <int HD, bool HILO, bool STARVE = false>
 cudaError_t launch_prompt(const PromptP &p, cudaStream_t st) {
     using C = Cfg<HD, HILO>;
-    cudaError_t e = g4_smem_optin((const void *)k_kv4_prompt<HD, HILO>, C::kSmem);
+    constexpr auto kernel = k_kv4_prompt<HD, HILO, STARVE>;
+    cudaError_t e = g4_smem_optin((const void *)kernel, C::kSmem);
     if (e != cudaSuccess) return e;
     static std::atomic<bool> fits{false};                       // a build with fewer registers would wait for more
     if (!fits) {
         cudaFuncAttributes a;
-        e = cudaFuncGetAttributes(&a, (const void *)k_kv4_prompt<HD, HILO>);
+        e = cudaFuncGetAttributes(&a, (const void *)kernel);
         if (e != cudaSuccess) return e;
         if (a.numRegs < kRegs) return cudaErrorLaunchOutOfResources;
         fits = true;
@@ -1003,7 +1032,7 @@ cudaError_t launch_prompt(const PromptP &p, cudaStream_t st) {
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = C::kCl > 1 ? 2 : 1;
-    e = cudaLaunchKernelEx(&cfg, k_kv4_prompt<HD, HILO>, p);
+    e = cudaLaunchKernelEx(&cfg, kernel, p);
     if (e != cudaSuccess || p.splits == 1) return e;
     return g4_launch(k_kv4_prompt_join<HD>, dim3((unsigned)p.slots * p.c.kv_heads, kM / 8), dim3(kJoinThreads), 0, st,
                      true, p);
@@ -1011,6 +1040,9 @@ cudaError_t launch_prompt(const PromptP &p, cudaStream_t st) {
 
 template <int HD>
 cudaError_t launch_hd(const PromptP &p, cudaStream_t st) {
+    if constexpr (HD >= 256)
+        if (p.starve) return p.type == G4_TYPE_F32 ? launch_prompt<HD, true, true>(p, st) : cudaErrorNotSupported;
+    if (p.starve) return cudaErrorNotSupported;
     return p.type == G4_TYPE_F32 ? launch_prompt<HD, true>(p, st) : launch_prompt<HD, false>(p, st);
 }
 
@@ -1042,7 +1074,8 @@ size_t kv4_prompt_ws(const Kv4View &c, int type, int q_heads) {
 }
 
 cudaError_t kv4_launch_prompt(const Kv4View &c, int type, int q_heads, const void *q, long long q_stride, void *out,
-                              long long out_stride, float scale, int window, void *ws, cudaStream_t st) {
+                              long long out_stride, float scale, int window, void *ws, int starve,
+                              cudaStream_t st) {
     PromptP p;
     p.c = c;
     p.type = type;
@@ -1054,6 +1087,7 @@ cudaError_t kv4_launch_prompt(const Kv4View &c, int type, int q_heads, const voi
     p.out_stride = out_stride;
     p.scale = scale;
     p.window = window;
+    p.starve = starve;
     p.parts = (float *)ws;
     p.stats = p.parts + (size_t)p.slots * c.kv_heads * p.splits * kM * c.hd;
     if (c.hd == 64) return launch_hd<64>(p, st);

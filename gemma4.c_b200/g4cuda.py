@@ -127,6 +127,7 @@ def load(path=LIB_PATH):
     L.g4_beam_workspace.argtypes = [C.c_int] * 3
     L.g4_beam_workspace.restype = u64
     L.g4_beam_select.argtypes = [C.c_int] * 4 + [vp, i64, vp, vp, C.c_int, vp, vp, vp, vp, vp, u64, vp]
+    L.g4_test_kv4_attention_starve.argtypes = [C.c_int]
     L.g4_kv4_reorder.argtypes = [cache] + [C.c_int] * 3 + [vp] * 4 + [C.c_int, vp, vp, vp]
     _lib = L
     return L

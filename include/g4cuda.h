@@ -358,6 +358,13 @@ int g4_launches_per_token(g4_ctx *ctx, int *n);
  * and later steps run normally. G4_ERR_STATE when persistent decode is off. */
 int g4_test_starve_next_step(g4_ctx *ctx);
 
+/* The same for g4_kv4_attention: in the next call of this process that launches
+ * it (fp32, 256 or 512 dimensions; G4_ERR_CUDA otherwise) the waits of its first
+ * CTA run out, by what is never copied or announced (1), or, with many rows per
+ * sequence, one counts as run out (2). That CTA's rows become NaN, the others
+ * stay what they are. 0 takes it back. */
+int g4_test_kv4_attention_starve(int what);
+
 /* ---- synthetic model images (benchmarks and parity tests) ----
  * A seeded random-init Gemma 4 E2B in the exact .bin layout gemma4.c reads. */
 uint64_t g4synth_image_bytes(void);
