@@ -7,9 +7,9 @@
 //   S = Q K^T   fp16 operands in shared memory, fp32 accumulator in TMEM
 //   O += P V    P (fp16) in TMEM as the A operand, V^T in shared memory
 // Operands: a key or value c * scale has 11 significant bits (8 of the scale, 3 of
-// the code), so as fp16 it is exact once the largest scale of the keys in work is
-// brought to a fixed power of two (of scales below 2^-11 of the largest, bits are lost
-// that are 2^-20 of the largest value at most). q is scaled per row by a power of two; an fp32 q
+// the code), so as fp16 it is exact once the largest scale of the keys in work (of values:
+// in their group of dimensions) is brought to a fixed power of two (of scales below 2^-11 of
+// the largest, bits are lost that are 2^-20 of the largest value at most). q is scaled per row by a power of two; an fp32 q
 // is split into high and low fp16 (22 bits; one fp16 holds a 16-bit q exactly), and so is
 // p for every type (one fp16 p, 11 bits, would show beside an fp16 output's own rounding).
 //
@@ -263,7 +263,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
     // 1 / power of two of each row's q: read by both threads of a row before they first meet,
     // and so before tile 1 writes here
     float *q_inv = pair[1][0];
-    __shared__ uint32_t k_top, v_top;                           // largest scales (bf16 bits) of the keys in work
+    __shared__ uint32_t k_top, v_top[G];                        // largest scales (bf16 bits) of the keys in work
     __shared__ int missing[4][4];                               // [tile % 4][record]: tile + 1 if its page is missing
     __shared__ int nan_tile[4];                                 // [tile % 4]: tile + 1 if a value of it is NaN
     __shared__ int2 nan_keys[4][G][4];                          // [tile % 4][group][record]: tile + 1, keys
@@ -300,9 +300,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
             mbar_init(&xfull[i], 1);
             mbar_init(&xfree[i], 1);
         }
-        k_top = v_top = 0;
+        k_top = 0;
         failed = 0;
     }
+    if (tid < G) v_top[tid] = 0;
     if (tid < 4) nan_tile[tid] = 0;
     if (tid < 16) missing[tid >> 2][tid & 3] = 0;
     if (tid < 16 * G) nan_keys[0][0][tid] = make_int2(0, 0);
@@ -392,7 +393,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
         // The largest scales: a warp takes every 16th record, 8 at a time in flight, K scales
         // of a token per lane in its lower half, G V scales per lane in the upper one.
         constexpr int kScan = kSoftWarps + kConvWarps, kFlight = 8;
-        uint32_t km = 0, vm = 0;
+        uint32_t km = 0;
         const bool is_v = lane >= 16;
         const int i16 = lane & 15, at_lane = 16 * HD + (is_v ? 32 * HG + rank * (32 * G) + i16 * (2 * G)
                                                               : i16 * (2 * HG) + rank * (2 * G));
@@ -426,18 +427,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
                 }
             }
         }
-        // K in the lower half of the warp, V in the upper one
-        vm = __reduce_max_sync(0xffffffffu, lane >= 16 ? km : 0);
-        km = __reduce_max_sync(0xffffffffu, lane >= 16 ? 0 : km);
-        if (lane == 0) {
-            atomicMax(&k_top, km);
-            atomicMax(&v_top, vm);
-        }
+        // K in the lower half of the warp, V in the upper one, 16 / G lanes a group
+#pragma unroll
+        for (int o = 1; o < 16 / G; o <<= 1) km = max(km, __shfl_xor_sync(0xffffffffu, km, o));
+        if (lane % (16 / G) == 0) atomicMax(is_v ? &v_top[i16 / (16 / G)] : &k_top, km);
     }
     __syncthreads();
-    // scales times 2^ka (2^va) are at most 2^12; an operand is then the value times 2^(ka - 17)
-    const int ka = k_top ? min(max(11 - ((int)(k_top >> 7) - 127), -100), 113) : 0;
-    const int va = v_top ? min(max(11 - ((int)(v_top >> 7) - 127), -100), 113) : 0;
+    // scales times 2^up are at most 2^12; an operand is then the value times 2^(up - 17). Values
+    // have a factor for each group of dimensions (columns of their own in the output).
+    auto up_of = [](uint32_t top) { return top ? min(max(11 - ((int)(top >> 7) - 127), -100), 113) : 0; };
+    const int ka = up_of(k_top);
 
     // A wait ran out: this thread waits no more, and the rows of both CTAs are NaN, whose
     // scores are made of both halves.
@@ -502,7 +501,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
         const int cw = warp - kSoftWarps, rec = cw & 3, g0 = cw >> 2;
         const bool busy = g0 < G;
         const int g = lane >> 2, t = lane & 3;
-        const float kup = pow2(ka), vup = pow2(va);
+        const float kup = pow2(ka);
+        float vup[NB];
+#pragma unroll
+        for (int n = 0; n < NB; n++) vup[n] = pow2(up_of(v_top[busy ? g0 + 2 * n : 0]));
         // the page of this warp's record of tile j (loaded an iteration before it is looked at),
         // and the record's address
         const int *table = p.c.table + (long long)it.seq * p.c.table_stride;
@@ -615,8 +617,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
 #pragma unroll
                     for (int pr = 0; pr < 2; pr++) {
                         const uint32_t sw = pr ? vs[n].y : vs[n].x;
-                        const float f0 = bound(__uint_as_float(sw << 16) * vup),
-                                    f1 = bound(__uint_as_float(sw & 0xffff0000u) * vup);
+                        const float f0 = bound(__uint_as_float(sw << 16) * vup[n]),
+                                    f1 = bound(__uint_as_float(sw & 0xffff0000u) * vup[n]);
                         const uint32_t s = pack_h(f0, f1), s16 = pack_h(f0 * 16.0f, f1 * 16.0f),
                                        off = mul_h(s, 0x84008400u);
                         const int key = rec * 16 + 8 * pr + 2 * t;          // keys key, key + 1
@@ -875,7 +877,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
         const long long item = blockIdx.x / CL;
         float *acc = sums();
         const float f = factor();
-        const float fac = pow2(min(17 - va, 127)) * (part ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l);
+        const float inv = part ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
         if (part && rank == 0 && half == 0) {
             p.stats[item * (2 * kM) + r] = m;
             p.stats[item * (2 * kM) + kM + r] = l;
@@ -901,6 +903,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
                 }
             }
             const bool bad = nans >> (c / kKv4Group) & 1;
+            const float fac = pow2(min(17 - up_of(v_top[c / kKv4Group]), 127)) * inv;
 #pragma unroll
             for (int x = 0; x < 32; x += 8) {
                 float y[8];

@@ -731,3 +731,30 @@ def test_attention_in_a_workspace_of_the_largest_call(g4, hd, kv, heads, name):
         out = torch.empty_like(want)
         s.attend(q, out, kind_of(g4, name), 0.1, 0, ws=ws[:n])
         assert torch.equal(out, want) and (ws[need:] == 0x5A).all()
+
+
+@pytest.mark.parametrize("hd,kv", [(128, 2), (256, 1), (512, 1)])
+@pytest.mark.parametrize("start", [0, 700])
+def test_prompt_tiles_groups_of_different_sizes(g4, hd, kv, start):
+    """Values whose groups of dimensions differ by up to 2^30: every group as exact as if it
+    were alone (the bound is the dimension's own)."""
+    rng = np.random.default_rng(hd + start)
+    rows = 150
+    s = Setup(g4, [(0, start + rows)], kv, hd, 64)
+    size = np.repeat(2.0 ** -np.array([0, 9, 18, 30, 14, 27, 5, 22][:hd // 64] * kv, np.float32), 64).reshape(kv, hd)
+    size[kv - 1] = size[kv - 1][::-1]                   # not the same in every head
+    k = tensors(rng, start + rows, kv, hd, torch.float32)
+    v = (tensors(rng, start + rows, kv, hd, torch.float32) * dev(size, torch.float32)).contiguous()
+    s.write(k, v, 0)
+    ks, vs = ref.stored(as64(k)), ref.stored(as64(v))
+    s.spans, s.offsets, s.rows = [(start, rows)], np.array([0, rows], np.int32), rows
+    s.upload()
+    for name in ("f32", "bf16"):
+        q = tensors(rng, rows, 8, hd, TYPES[name])
+        out = torch.empty_like(q)
+        s.attend(q, out, kind_of(g4, name), 0.1, 0)
+        q64, got = as64(q), as64(out)
+        for row in range(rows):
+            want, mag, delta, n = ref.attention(q64[row], ks, vs, start + row, 0.1, 0)
+            tol = ref.tolerance(want, mag, delta, n, torch.finfo(TYPES[name]).eps)
+            assert (np.abs(got[row] - want) <= tol).all(), (name, row)
