@@ -217,6 +217,19 @@ def cpu_reference_decode(img, max_seconds=10.0, max_steps=256, prompt=PREFILL):
         m.close()
 
 
+def cpu_baseline(img):
+    """The line's `cpu_baseline`: the reference's own rate here, or why there is none (its
+    library is built from its sources, which a machine need not have)."""
+    try:
+        cb = cpu_reference_decode(img)
+    except FileNotFoundError as e:
+        return {"unavailable": str(e)}
+    return {"value": cb["decode_tok_s"], "unit": "tok/s", "cores": cb["cores"], "kind": "reference",
+            "sample": f"{cb['steps']} decode steps ({cb['seconds']:.1f} s) after a "
+                      f"{PREFILL}-token prefill, {cb['variant']} build",
+            "prefill_tok_s_512": cb["prefill_tok_s"]}
+
+
 def run_reference_arm(args, dist):
     """--impl reference: the reference's own CPU implementation of the path on
     this host's cores (rank 0 only), same metric and workload. Only the
@@ -229,7 +242,11 @@ def run_reference_arm(args, dist):
     sys.path.insert(0, os.path.join(ROOT, "oracle"))
     from oracle import Reference
     Reference.use_all_cores()
-    ref = Reference()
+    try:
+        ref = Reference()
+    except FileNotFoundError as e:
+        print(json.dumps({"impl": "reference", "unavailable": str(e)}), flush=True)
+        return
     img = ref.synth_image(seed=0, flags=0)
     m = ref.open_model(img)
     ids = prompt_ids(PREFILL)
@@ -605,12 +622,7 @@ def run_ours(args, dist):
         line["clocks"] = clk
     m.close()
     if dist.rank == 0 and dist.world == 1 and not args.no_cpu_baseline:
-        cb = cpu_reference_decode(img)
-        line["cpu_baseline"] = {"value": cb["decode_tok_s"], "unit": "tok/s", "cores": cb["cores"],
-                                "kind": "reference",
-                                "sample": f"{cb['steps']} decode steps ({cb['seconds']:.1f} s) after a "
-                                          f"{PREFILL}-token prefill, {cb['variant']} build",
-                                "prefill_tok_s_512": cb["prefill_tok_s"]}
+        line["cpu_baseline"] = cpu_baseline(img)
     if dist.rank == 0:
         print(json.dumps(line), flush=True)
 
