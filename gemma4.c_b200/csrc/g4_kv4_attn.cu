@@ -16,17 +16,20 @@
 //   S^T = K Q^T  fp16. A nibble n = c + 8 in the low bits of an fp16 is the
 //                subnormal n 2^-24 (16 n 2^-24 one nibble up): one AND makes two
 //                operands. The 8 is taken off in the accumulator's start value,
-//                -8 sum(q). q is scaled per row to 2^13..2^14 and, if fp32, split
-//                into high and low halves (22 bits).
+//                -8 sum(q), whose truncation is the same for every key (codes without
+//                the 8: outputs 4.8e-6 off, with it 2.4e-6). q is scaled per row to
+//                2^13..2^14 and, if fp32, split into high and low halves (22 bits),
+//                each with an accumulator of its own: the tensor core truncates by the
+//                size of the sum (in one: 3.5e-6; 1 % of a 64-sequence step).
 //   O^T = V^T P^T  bf16, whose range needs no common factor over the scales. A
 //                nibble is the bf16 subnormal n 2^-133 (16 n 2^-133 one nibble up);
 //                a packed add takes the 8 off, because the accumulator runs over all
 //                keys and an offset there would add up the truncations of the tensor
 //                core. p is 2^80 times too large to keep sums away from 2^-126: values
 //                up to 2^38 times a code are safe. p vs is split into high and low
-//                bf16: for fp32 outputs from the fp32 product (2^-18 of it is lost; with
-//                the next form outputs were 6.8e-6 off instead of 4.1e-6, a 64-sequence
-//                step took 2 % less), for others by packed FMAs on p's own halves (16 bits).
+//                bf16: for fp32 outputs from the fp32 product (2^-18 of it is lost, a
+//                third of what they are off; a third term would take 5 % longer), for
+//                others by packed FMAs on p's own halves (16 bits).
 // Every warp streams its own records of 16 keys through a ring in shared memory
 // and keeps its own running maximum, sum and output; the warps meet once per
 // sequence and head. Work is counted in records over all (sequence, row tile, kv
@@ -57,7 +60,7 @@ constexpr int kSms = 148;
 constexpr int kJoinThreads = 512;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 8.0f;                      // log2 of how far p may pass 1
-constexpr float kUp = 80.0f;                        // p is 2^80 times too large
+constexpr float kUp = 0x1p80f;                      // p is 2^80 times too large
 constexpr float kEven = 0x1p53f, kOdd = 0x1p49f;    // outputs: 2^133 / 2^80, 16 times less for odd dimensions
 
 template <int HD>
@@ -537,7 +540,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kOcc) k_kv4_attn(const __gr
                          const uint32_t (&k1s)[(G + 1) / 2], float (&sc)[4]) {
             const uint4 kc = *reinterpret_cast<const uint4 *>(rec + gr * 512 + lane * 16);
             const float2 q0 = *reinterpret_cast<const float2 *>(qoff + gr * 8 + 2 * t);
-            float d[4] = {q0.x, q0.y, q0.x, q0.y};
+            float d[4] = {q0.x, q0.y, q0.x, q0.y}, dl[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int half = 0; half < 2; half++) {
                 uint32_t x = half ? kc.y : kc.x, z = half ? kc.w : kc.z;
@@ -547,12 +550,16 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kOcc) k_kv4_attn(const __gr
                 if (HILO) bl = qlo[qi];
                 const uint32_t a0 = x & 0x000f000fu, a1 = z & 0x000f000fu, a2 = x & 0x00f000f0u, a3 = z & 0x00f000f0u;
                 mma_h(d, a0, a1, a2, a3, bh.x, bh.y);
-                if (HILO) mma_h(d, a0, a1, a2, a3, bl.x, bl.y);
+                if (HILO) mma_h(dl, a0, a1, a2, a3, bl.x, bl.y);
                 x >>= 8;
                 z >>= 8;
                 const uint32_t a4 = x & 0x000f000fu, a5 = z & 0x000f000fu, a6 = x & 0x00f000f0u, a7 = z & 0x00f000f0u;
                 mma_h(d, a4, a5, a6, a7, bh.z, bh.w);
-                if (HILO) mma_h(d, a4, a5, a6, a7, bl.z, bl.w);
+                if (HILO) mma_h(dl, a4, a5, a6, a7, bl.z, bl.w);
+            }
+            if (HILO) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) d[i] += dl[i];
             }
             const float k0 = half_of(k0s[gr / 2], gr & 1), k1 = half_of(k1s[gr / 2], gr & 1);
             sc[0] = fmaf(d[0], k0, sc[0]);
@@ -581,8 +588,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kOcc) k_kv4_attn(const __gr
                 const uint32_t ab = __byte_perm(vc.x, vc.y, j < 2 ? 0x5410 : 0x7632) >> (8 * (j & 1));
                 const uint32_t cd = __byte_perm(vc.z, vc.w, j < 2 ? 0x5410 : 0x7632) >> (8 * (j & 1));
                 const uint32_t a0 = code_lo(ab), a1 = code_hi(ab), a2 = code_lo(cd), a3 = code_hi(cd);
-                mma_b(o[gr][j], a0, a1, a2, a3, h0, h1);
                 mma_b(o[gr][j], a0, a1, a2, a3, l0, l1);
+                mma_b(o[gr][j], a0, a1, a2, a3, h0, h1);
             }
         };
 
@@ -642,11 +649,14 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kOcc) k_kv4_attn(const __gr
                             o[i][j][3] *= al1;
                         }
                 }
-                const float mref = (m == -INFINITY ? 0.0f : m) - kUp;
+                const float mref = m == -INFINITY ? 0.0f : m;
                 float pr[4];
 #pragma unroll
                 for (int i = 0; i < 4; i++) pr[i] = ex2(fmaf(sc[i], rs, -mref));
                 l += (pr[0] + pr[1]) + (pr[2] + pr[3]);
+                // (not 80 more in the exponent, which would round it to 2^-18)
+#pragma unroll
+                for (int i = 0; i < 4; i++) pr[i] *= kUp;
                 if constexpr (HILO) {
                     p01 = pk(pr[0], pr[1]);
                     p23 = pk(pr[2], pr[3]);
@@ -673,7 +683,6 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD>::kOcc) k_kv4_attn(const __gr
         }
         l += __shfl_xor_sync(0xffffffffu, l, 1);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
-        l *= 0x1p-80f;
         if (t == 0) { sm_m[stream][g] = m; sm_l[stream][g] = l; }
         __syncwarp();
         float *ow = reinterpret_cast<float *>(my_ring);

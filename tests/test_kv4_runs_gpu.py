@@ -168,3 +168,32 @@ def test_unwritten_scales_behind_large_tiles(g4, bits):
         s = Setup(g4, [(40, 75)], 1, hd, 64, fill=fill)
         assert ranges_of(g4, s, 8, "f32") > 0
         check_attention(g4, s, 8, "f32", 0.1, 0, np.random.default_rng(6))
+
+
+@pytest.mark.parametrize("hd,span", [(512, (131000, 1)), (256, (131000, 2))])
+def test_error_of_fp32_outputs(g4, hd, span):
+    """fp32 outputs over long contexts are within 2^-18 of 64 bits in the 2-norm (random keys and
+    queries: errors of single keys are independent, so they add in squares). Few rows: p vs as two
+    bf16 terms is off by up to 2^-18, evenly spread: 2^-18 / sqrt(3) = 2.2e-6. A group's score is
+    four tensor-core steps that truncate by up to 2^-23 of 8 |sum q| = 64 (q of size 1): 64 2^-23
+    sqrt(4 / 12), times a scale of 0.37, sqrt(8) groups and 2 / sqrt(512): 4e-7. Up to 14 steps of an
+    output, each up to 2^-23 of it and always towards 0: 14 2^-24 = 8e-7. In squares 2.4e-6."""
+    start, rows = span
+    heads, n, scale = 8, start + rows, 2 / np.sqrt(hd)
+    s = Setup(g4, [(0, n)], 1, hd, 64, fill=0)
+    g = torch.Generator(device="cuda:0").manual_seed(hd + rows)
+    k, v = (torch.randn((n, 1, hd), generator=g, device="cuda:0") for _ in range(2))
+    s.write(k, v, 0)
+    s.read(k, v, 0)                                     # codes times scales: exact in fp32
+    s.spans, s.offsets, s.rows = [span], np.array([0, rows], np.int32), rows
+    s.upload()
+    q = torch.randn((rows, heads, hd), generator=g, device="cuda:0")
+    out = torch.empty_like(q)
+    s.attend(q, out, 0, scale, 0)
+    hidden = torch.arange(n, device="cuda:0") > torch.arange(start, n, device="cuda:0")[:, None]
+
+    exact = torch.empty(q.shape, dtype=torch.float64, device="cuda:0")
+    for h in range(heads):
+        sc = (q[:, h].double() @ k[:, 0].double().T * scale).masked_fill(hidden, float("-inf"))
+        exact[:, h] = torch.softmax(sc, -1) @ v[:, 0].double()
+    assert float((out.double() - exact).norm() / exact.norm()) <= 2.0 ** -18
