@@ -482,11 +482,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const __grid_constan
                     wait(&kfull, j + 2);
                     tc_fence_after();
                     const uint32_t d = tmem + kColS + (j & 1) * kT;
+                    // the low halves of q first: the tensor cores truncate by the size of the sum
+                    // (fp32 outputs of a chunk at 16384 keys 5.0e-6 off, now 3.3e-6)
 #pragma unroll
                     for (int half = 0; half < (HILO ? 2 : 1); half++)
 #pragma unroll
                         for (int i = 0; i < G * 4; i++)
-                            mma_f16(d, umma_desc((half ? ql : qh) + (i >> 2) * (kM * 128), (i & 3) * 32),
+                            mma_f16(d, umma_desc((HILO && !half ? ql : qh) + (i >> 2) * (kM * 128), (i & 3) * 32),
                                     umma_desc(kb + (i >> 2) * (kT * 128), (i & 3) * 32), kIdS, half || i);
                     mma_commit(&sfull[j & 1]);
                 }

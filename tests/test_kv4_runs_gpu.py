@@ -170,14 +170,19 @@ def test_unwritten_scales_behind_large_tiles(g4, bits):
         check_attention(g4, s, 8, "f32", 0.1, 0, np.random.default_rng(6))
 
 
-@pytest.mark.parametrize("hd,span", [(512, (131000, 1)), (256, (131000, 2))])
+@pytest.mark.parametrize("hd,span", [(512, (131000, 1)), (256, (131000, 2)), (512, (16000, 384)), (256, (16000, 300))])
 def test_error_of_fp32_outputs(g4, hd, span):
     """fp32 outputs over long contexts are within 2^-18 of 64 bits in the 2-norm (random keys and
     queries: errors of single keys are independent, so they add in squares). Few rows: p vs as two
     bf16 terms is off by up to 2^-18, evenly spread: 2^-18 / sqrt(3) = 2.2e-6. A group's score is
     four tensor-core steps that truncate by up to 2^-23 of 8 |sum q| = 64 (q of size 1): 64 2^-23
     sqrt(4 / 12), times a scale of 0.37, sqrt(8) groups and 2 / sqrt(512): 4e-7. Up to 14 steps of an
-    output, each up to 2^-23 of it and always towards 0: 14 2^-24 = 8e-7. In squares 2.4e-6."""
+    output, each up to 2^-23 of it and always towards 0: 14 2^-24 = 8e-7. In squares 2.4e-6. Many rows:
+    16 steps of the high halves of q truncate a score of up to 8 by half of 2^-23 of what has been
+    summed up, half of it on the average: 16 / 4 2^-23 8 = 3.8e-6 of p at most, for all keys in the same
+    direction, of which the output's norm keeps the deviation from its mean (a half); 128 steps of an
+    output between sums: 128 / 4 2^-23 = 3.8e-6 where all values have one sign, less by the same reason.
+    In squares 3e-6."""
     start, rows = span
     heads, n, scale = 8, start + rows, 2 / np.sqrt(hd)
     s = Setup(g4, [(0, n)], 1, hd, 64, fill=0)
