@@ -513,6 +513,11 @@ int g4_beam_select(int groups, int beams, int vocab, int type, const void *logit
     if (eos >= vocab || (eos < 0 && finished)) return G4_ERR_INVALID;
     if (((uintptr_t)workspace & 15) || workspace_bytes < g4_beam_workspace(groups, beams, vocab))
         return G4_ERR_INVALID;
+    // a group's CTA reads scores and flags while others, and its own threads, write theirs
+    const size_t n = (size_t)groups * beams;
+    const struct { const void *p; size_t n; } out[4] = {{out_scores, 4 * n}, {parents, 4 * n}, {tokens, 4 * n}, {out_finished, n}};
+    for (const auto &x : out)
+        if (kv4_overlap(x.p, x.n, scores, 4 * n) || kv4_overlap(x.p, x.n, finished, n)) return G4_ERR_INVALID;
     if (groups == 0) return G4_OK;
     DeviceOf dev(logits);
     if (dev.status() != G4_OK) return dev.status();

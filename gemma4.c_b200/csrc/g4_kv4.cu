@@ -537,10 +537,10 @@ int g4_kv4_reorder(const g4_kv4_cache *caches, int layers, int groups, int beams
         !aligned4(spare_in) || !aligned4(spare_out))
         return G4_ERR_INVALID;
     const long long rows = (long long)groups * beams;
-    const uintptr_t tb = (uintptr_t)rows * table_stride * 4, sb = (uintptr_t)rows * 4;
-    const uintptr_t ti = (uintptr_t)table_in, to = (uintptr_t)table_out, si = (uintptr_t)spare_in,
-                    so = (uintptr_t)spare_out;
-    if ((ti < to + tb && to < ti + tb) || (si < so + sb && so < si + sb)) return G4_ERR_INVALID;
+    const size_t tb = (size_t)rows * table_stride * 4, sb = (size_t)rows * 4;
+    const struct { const void *p; size_t n; } in[4] = {{table_in, tb}, {spare_in, sb}, {parents, sb}, {lengths, (size_t)groups * 4}};
+    for (const auto &x : in)
+        if (kv4_overlap(table_out, tb, x.p, x.n) || kv4_overlap(spare_out, sb, x.p, x.n)) return G4_ERR_INVALID;
     ReorderArgs a;
     for (int l = 0; l < layers; l++) {
         if (kv4_check_cache(&caches[l]) != G4_OK || caches[l].page_size != caches[0].page_size ||

@@ -100,6 +100,10 @@ int kv4_view(const g4_kv4_cache *c, const g4_kv4_batch *b, Kv4View *v);
 // type is known and rows of `heads` heads start every `stride` elements, 16-byte aligned
 bool kv4_tensor_ok(const void *p, int64_t stride, int heads, int hd, int type);
 size_t kv4_type_bytes(int type);
+// whether [a, a + an) and [b, b + bn) have a byte in common
+inline bool kv4_overlap(const void *a, size_t an, const void *b, size_t bn) {
+    return a && b && an && bn && (uintptr_t)a < (uintptr_t)b + bn && (uintptr_t)b < (uintptr_t)a + an;
+}
 
 // Makes the device that holds `p` current for a scope; ok() is false when one
 // of the pointers is not device memory of that device.

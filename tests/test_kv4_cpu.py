@@ -167,6 +167,32 @@ def test_reorder_refusals(g4):
     assert call(g=0) == 0
 
 
+def test_outputs_over_inputs_are_refused(g4):
+    """Outputs that share a byte with an input: refused; next to it: not."""
+    f, r = g4.load().g4_beam_select, g4.load().g4_kv4_reorder
+
+    def beam(**kw):
+        a = dict(s=P, fin=P + 0x100, os=P + 0x200, pa=P + 0x300, to=P + 0x400, fo=P + 0x500) | kw
+        return f(2, 4, 1000, 0, P + 0x1000, 1000, a["s"], a["fin"], 3, a["os"], a["pa"], a["to"], a["fo"], P, 1 << 40,
+                 None)
+
+    def reorder(**kw):
+        a = dict(pa=P, le=P + 0x100, ti=P + 0x200, to=P + 0x400, si=P + 0x600, so=P + 0x700) | kw
+        return r(g4.kv4_caches([cache(g4)]), 1, 2, 4, a["pa"], a["le"], a["ti"], a["to"], 4, a["si"], a["so"], None)
+    for kw in (dict(os=P), dict(os=P + 28), dict(os=P - 28), dict(pa=P + 0x100 + 4), dict(to=P + 4), dict(fo=P + 0x100),
+               dict(fo=P + 0x100 + 7), dict(fo=P + 31)):
+        assert beam(**kw) == -1, kw
+    for kw in (dict(to=P), dict(to=P + 0x600 - 124), dict(so=P + 0x200 + 124), dict(so=P + 28), dict(so=P + 0x104),
+               dict(to=P + 0x200), dict(so=P + 0x600), dict(to=P + 0x100 + 4)):
+        assert reorder(**kw) == -1, kw
+    torch = pytest.importorskip("torch")
+    if not torch.cuda.is_available():                   # the addresses are nobody's
+        for kw in (dict(), dict(os=P + 32), dict(fo=P + 0x100 + 8)):
+            assert beam(**kw) != -1, kw
+        for kw in (dict(), dict(so=P + 32), dict(to=P + 0x200 + 128)):
+            assert reorder(**kw) != -1, kw
+
+
 def test_reference_layout_is_a_bijection():
     """Every nibble and scale of a record belongs to one token and dimension."""
     rng = np.random.default_rng(0)
