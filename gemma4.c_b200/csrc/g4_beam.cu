@@ -108,7 +108,7 @@ G4_DEV float ex2(float x) {
 // in flight in registers while it works on one; the CTA's threads meet in chunks 0,
 // 1, 2, 4, ... for a threshold that few values pass. The pass is bound by its
 // instructions (14 a value) as much as by HBM: 128 rows of 262144 in fp32 take 30 us
-// (4.5 TB/s), in bf16 the same. Measured beside it (with the merge, 35 us): 32 values a
+// (4.5 TB/s), in bf16 the same. Measured beside it (with the merge, 36 us): 32 values a
 // thread and chunk 41 us, five CTAs an SM 37 us, two waves of shorter slices 37 us,
 // rings of 48 KB in shared memory filled by cp.async 39 us.
 // A slice whose first chunk is one value throughout (masked) has that value for its

@@ -22,10 +22,10 @@
 // codes in flight in registers), 16 the MMAs. S and P are double-buffered: while the softmax works on tile
 // j, the MMAs of P_{j-1} V and S_{j+1} run and K of tile j + 2 and V of tile j are converted.
 //
-// Measured: 512 tokens of 8 fp32 heads of 512 dimensions behind 15872 450 us (301 TFLOP/s
+// Measured: 512 tokens of 8 fp32 heads of 512 dimensions behind 15872 451 us (300 TFLOP/s
 // of the operator's, twice that on the tensor cores, which work on two terms of q and of
-// p); 2048 tokens of 256 dimensions behind 6144 293 us (410); 2048 tokens of 32 bf16 heads
-// of 128 dimensions, 8 kv heads, 108 us (318). A tile takes 3.2 us at 512 dimensions, where
+// p); 2048 tokens of 256 dimensions behind 6144 297 us (405); 2048 tokens of 32 bf16 heads
+// of 128 dimensions, 8 kv heads, 110 us (312). A tile takes 3.2 us at 512 dimensions, where
 // the MMAs need 1.4 and sending the halves of S (32 KB each way, st.async; plain remote
 // stores with one arrival a warp 522 us, sending before the maximum 463 us) bounds it; 2.1 us
 // at 256, where MMAs of 64 columns (48 clocks against 32 for their share) bound it.
@@ -69,9 +69,10 @@ struct Cfg {
     static constexpr int kK = G * kT * 128;
     static constexpr int kV = kDc * 128;                     // V^T: rows are dimensions, 64 keys
     // The tensor cores truncate as they add up, 8 steps a tile: an error that grows with
-    // the length of a run (fp32, 128 tiles: 2e-5 of the output, 4e-5 where values have one
-    // sign; after 32 tiles 5.5e-6 and 9e-6, after 16 3.3e-6 and 4.3e-6). So O is added to a
-    // sum in memory, in fp32, after every kRun tiles: 5 % of a chunk's time (32 tiles: 1 %).
+    // the length of a run (fp32, 128 tiles: 2e-5 of the output, 5e-5 where values have one
+    // sign; after 32 tiles 5.3e-6 and 1.1e-5, after 16 3.3e-6 and 5.6e-6). So O is added to a
+    // sum in memory, in fp32, after every kRun tiles (chunk of 512 tokens at 16384 without
+    // sums 414 us, every 32 tiles 438, every 16 451).
     // 16-bit outputs round by more than that up to 256.
     static constexpr int kRun = HILO ? 16 : 256;
     static constexpr int kX = kCl > 1 ? kM * kT * 4 : 0;     // the other CTA's half of S

@@ -178,11 +178,10 @@ def test_error_of_fp32_outputs(g4, hd, span):
     four tensor-core steps that truncate by up to 2^-23 of 8 |sum q| = 64 (q of size 1): 64 2^-23
     sqrt(4 / 12), times a scale of 0.37, sqrt(8) groups and 2 / sqrt(512): 4e-7. Up to 14 steps of an
     output, each up to 2^-23 of it and always towards 0: 14 2^-24 = 8e-7. In squares 2.4e-6. Many rows:
-    16 steps of the high halves of q truncate a score of up to 8 by half of 2^-23 of what has been
-    summed up, half of it on the average: 16 / 4 2^-23 8 = 3.8e-6 of p at most, for all keys in the same
-    direction, of which the output's norm keeps the deviation from its mean (a half); 128 steps of an
-    output between sums: 128 / 4 2^-23 = 3.8e-6 where all values have one sign, less by the same reason.
-    In squares 3e-6."""
+    128 steps of an output between two sums, each of which cuts off half of 2^-24 to 2^-23 (on the
+    average 0.375 2^-23) of a sum of random values, which grows like a root (2/3 on the average): 128
+    2/3 0.375 2^-23 = 3.8e-6 = 2^-18. Beside it the 16 steps of the high halves of q, which shrink a
+    score of size 2 by 16 / 4 2^-23 of itself (1e-6), hardly count in squares."""
     start, rows = span
     heads, n, scale = 8, start + rows, 2 / np.sqrt(hd)
     s = Setup(g4, [(0, n)], 1, hd, 64, fill=0)
