@@ -184,11 +184,11 @@ int g4_kv4_read(const g4_kv4_cache *cache, const g4_kv4_batch *batch, int type, 
  * with window > 0 only those above p - window: out = softmax(scale * q.k) v.
  * A row that sees no key (padding, no pages) gets 0; rows from offsets[n] on
  * are left as they were. Scores, softmax statistics and sums are fp32; q keeps
- * 22 significant bits, the probabilities 16 or more; scores must stay in fp32's range
- * and values below 2^38. Calls with many rows per sequence hold keys and values
- * to 2^-20 of the largest that 128 of their rows see (values: of the largest in
- * their group of 64 dimensions), others exactly. A NaN in a
- * key or a query makes the rows that see it NaN, in a value their group of 64
+ * 22 significant bits, the probabilities 16 or more; scores must stay in fp32's
+ * range, queries below 2^116 and values below 2^38. Calls with many rows per
+ * sequence hold keys and values to 2^-20 of the largest that 128 of their rows see
+ * (values: of the largest in their group of 64 dimensions), others exactly. A NaN
+ * in a key or a query makes the rows that see it NaN, in a value their group of 64
  * dimensions. A wait inside a kernel that runs out (2 s) makes its rows NaN too.
  * `workspace` (g4_kv4_attention_workspace bytes, 16-byte aligned, any content)
  * is scratch of this call alone: calls that may overlap on the GPU (other
